@@ -44,6 +44,7 @@ extern "C" {
 #define SM_ERR_BAD_EXPERT 201
 #define SM_ERR_BAD_RETURN_ROW 202 /* home-down EP: an up-projection row with no valid home row */
 #define SM_ERR_BAD_COUNT 203      /* EP with device-side counts: a count outside the exchange buffers */
+#define SM_ERR_BAD_TOKEN 204      /* an explicit routing list names a token outside [0, T) */
 
 /* Message describing the calling thread's most recent non-zero return. */
 const char* sm_last_error(void);
@@ -466,6 +467,60 @@ int sm_set_gemm_sm_reserve(int n);
  * into *err (if it held 0) and the kernel returns, leaving the context usable -- the same path by
  * which a lost arrival inside a GEMM becomes an error status instead of a hung GPU. */
 int sm_selftest_bounded_wait(int32_t* err, void* stream);
+
+/*
+ * Switch balance loss of the router with the per-expert counts (reference sonicmoe/moe.py:263-276).
+ *   p = softmax(router_logits[t]), P_e = sum of p[t][e] over the tokens that count, n = sum P,
+ *   f = the experts' counts, F = sum f:   *loss = E * sum_e (P_e / n) (f_e / F)   (0 when n or F is 0).
+ *   router_logits [T, E] (dtype SM_DTYPE_*).  token_mask [T] bytes, or NULL: tokens with 0 do not count
+ *   (their logits are not read).  Exactly one of
+ *     topk_indices [T, K] int32, K >= 1: f is counted here over the tokens that count, into
+ *       expert_frequency_out [E]; an index outside [0, E) is not counted and sets err to 201;
+ *     expert_frequency [E] int32, with K = 0: f as given (expert_frequency_out NULL, or receives a copy).
+ *   coef [E] float32 receives what sm_switch_loss_bwd needs.  The sums are added in a fixed order: the
+ *   same inputs give the same bits.  err may be NULL.
+ */
+size_t sm_switch_loss_workspace(int T, int E);
+int sm_switch_loss(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                   const int32_t* topk_indices, int K, const int32_t* expert_frequency, float* loss, float* coef,
+                   int32_t* expert_frequency_out, void* workspace, size_t workspace_bytes, int32_t* err,
+                   void* stream);
+/* dlogits [T, E] (the logits' dtype) = *dloss * dloss/dlogits; rows of tokens that do not count are 0. */
+int sm_switch_loss_bwd(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                       const float* coef, const float* dloss, void* dlogits, void* stream);
+
+/*
+ * 4-bit expert weights.  w [E, N, K] bf16 (N, K multiples of 8; N = 2I rows gate/up interleaved, or with
+ * concat_glu gate rows then up rows) becomes codes in [-7, 7] and one scale per `group` (32, 64 or 128)
+ * columns of a row: the smallest number of 5 significant bits (at least 2^-126) that is >= amax / 7;
+ * code = w / scale to nearest, ties to even.  Every code times its scale is exactly a bf16 number.
+ * wq [sm_int4_weight_bytes] and scales [sm_int4_scale_count] bf16 are in this library's own order
+ * (16-byte aligned).  A group holding an infinity or NaN gets a NaN scale.
+ */
+size_t sm_int4_weight_bytes(int E, int N, int K);
+size_t sm_int4_scale_count(int E, int N, int K, int group);
+int sm_weight_prep_int4(const void* w, int E, int N, int K, int group, int concat_glu, uint8_t* wq, void* scales,
+                        void* stream);
+/* The bf16 weights [E, N, K], in the caller's row order, that a prepared 4-bit weight stands for (exact). */
+int sm_int4_expand(const uint8_t* wq, const void* scales, int E, int N, int K, int group, int concat_glu, void* w,
+                   void* stream);
+
+/*
+ * MoE layer forward on 4-bit expert weights: out[t] = sum over t's entries (expert e, score s) of
+ * s * W2_e (silu(W1_e^gate x_t) * (W1_e^up x_t)), x and out bf16 [T, H], no quantisation of x; the
+ * entries' sum is added in fp32 in entry order (the same inputs give the same bits).
+ *   K >= 1, token_indices NULL: top-k arrays [T, K], n_entries = T*K, entry f belongs to token f / K;
+ *   K = 0: explicit lists of n_entries, token_indices sorted ascending.
+ *   w1q / w2q: sm_weight_prep_int4 of [E, 2I, H] / [E, H, I].  H and I multiples of 8.
+ * expert_frequency [E] receives the entries per expert.  An entry whose expert is outside [0, E) or
+ * whose token is outside [0, T) contributes nothing and sets err (201 / 204); err may be NULL.
+ */
+size_t sm_moe_int4_workspace_bytes(int T, int n_entries, int H, int I, int E);
+int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_entries, const float* scores,
+                        const int32_t* token_indices, const int32_t* expert_indices, const uint8_t* w1q,
+                        const void* w1_scales, int w1_group, const uint8_t* w2q, const void* w2_scales, int w2_group,
+                        void* out, int32_t* expert_frequency, void* workspace, size_t workspace_bytes, int32_t* err,
+                        void* stream);
 
 #ifdef __cplusplus
 }

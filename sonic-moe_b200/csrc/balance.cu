@@ -1,0 +1,452 @@
+// Switch balance loss of the router (reference sonicmoe/moe.py:263-276), its per-expert counts and its
+// gradient.
+//
+//   p[t, :] = softmax(logits[t, :]),  P_e = sum_t p[t, e] over the tokens that count, n = sum_e P_e,
+//   f_e = entries routed to expert e, F = sum_e f_e,      loss = E * sum_e (P_e / n) (f_e / F)
+//   dloss/dlogits[t, e] = p[t, e] (c_e - sum_j p[t, j] c_j),   c_e = (E f_e - F) / (F n)
+//
+// (sum_e p[t, e] = 1, so neither the normalisation of P by n nor a constant added to c changes the
+// gradient; taking E f_e - F in integers instead of E f_e keeps c free of the cancellation that a
+// nearly balanced routing would otherwise bring.)
+//
+// switch_loss_kernel        one pass over the logits: softmax of each row in registers, its columns
+//                           summed per thread, then over the CTA; counts of the top-k indices beside it.
+// switch_loss_finish_kernel adds the CTAs' sums in a fixed order (no floating-point atomics: the loss
+//                           is the same bits every time) and forms the loss and c.
+// switch_loss_bwd_kernel    reads the logits once more, recomputes the softmax, writes the gradient.
+#include "common.cuh"
+#include "sonic_internal.h"
+
+namespace smb {
+
+namespace {
+
+constexpr int kSlThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_f32(float v, float* p) { *p = v; }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __half* p) { *p = __float2half_rn(v); }
+
+// 8 consecutive values; vec: how many of them one aligned access may cover (8, 4 or 1).
+template <typename InT>
+__device__ __forceinline__ void load8(const InT* __restrict__ src, int vec, int n, float* v) {
+  alignas(16) InT raw[8];
+  if (vec >= 4 && n >= 8) {
+    if constexpr (sizeof(InT) == 4) {
+      *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(src));
+      *reinterpret_cast<uint4*>(raw + 4) = __ldg(reinterpret_cast<const uint4*>(src + 4));
+    } else if (vec == 8) {
+      *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(src));
+    } else {
+      *reinterpret_cast<uint2*>(raw) = __ldg(reinterpret_cast<const uint2*>(src));
+      *reinterpret_cast<uint2*>(raw + 4) = __ldg(reinterpret_cast<const uint2*>(src + 4));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(raw[j]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(src[j]) : -__int_as_float(0x7f800000);
+}
+
+template <typename InT>
+__device__ __forceinline__ void store8(InT* __restrict__ dst, int vec, int n, const float* v) {
+  alignas(16) InT raw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) from_f32(v[j], &raw[j]);
+  if (vec >= 4 && n >= 8) {
+    if constexpr (sizeof(InT) == 4) {
+      reinterpret_cast<uint4*>(dst)[0] = *reinterpret_cast<uint4*>(raw);
+      reinterpret_cast<uint4*>(dst)[1] = *reinterpret_cast<uint4*>(raw + 4);
+    } else if (vec == 8) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(raw);
+    } else {
+      reinterpret_cast<uint2*>(dst)[0] = *reinterpret_cast<uint2*>(raw);
+      reinterpret_cast<uint2*>(dst)[1] = *reinterpret_cast<uint2*>(raw + 4);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) dst[j] = raw[j];
+}
+
+// Reductions over the L lanes that share a row: lanes of one warp (L <= 32) or the whole CTA, whose
+// partial results go through s_red.  Every thread of the group gets the result.
+template <int L, bool kMax>
+__device__ __forceinline__ float row_reduce(float x, float* s_red) {
+#pragma unroll
+  for (int o = (L < 32 ? L : 32) / 2; o >= 1; o >>= 1) {
+    const float y = __shfl_xor_sync(0xffffffffu, x, o);
+    x = kMax ? fmaxf(x, y) : x + y;
+  }
+  if constexpr (L > 32) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = s_red[0];
+#pragma unroll
+    for (int w = 1; w < L / 32; ++w) x = kMax ? fmaxf(x, s_red[w]) : x + s_red[w];
+  }
+  return x;
+}
+
+// The softmax of one row held as 8 * C values a lane: v becomes exp2(log2e (x - max)), the return
+// value 1 / sum.  The maximum is subtracted before the scaling, so that a row of the type's lowest
+// values does not overflow.  A row whose maximum is not finite (all -inf, or +inf or NaN in it) gives
+// NaN, as a softmax does.
+template <int L, int C>
+__device__ __forceinline__ float softmax_row(float (&v)[8 * C], float* s_red) {
+  float mx = v[0];
+#pragma unroll
+  for (int i = 1; i < 8 * C; ++i) mx = fmaxf(mx, v[i]);
+  mx = row_reduce<L, true>(mx, s_red);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8 * C; ++i) {
+    v[i] = ex2((v[i] - mx) * kLog2e);
+    s += v[i];
+  }
+  return 1.0f / row_reduce<L, false>(s, s_red);
+}
+
+// Lane layout: group lane l holds columns 8 l + 8 L c + (0..7), c < C; E <= 8 L C.
+template <typename InT, int L, int C>
+__device__ __forceinline__ void load_row(const InT* __restrict__ row, int E, int vec, int gl, float (&v)[8 * C]) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) load8<InT>(row + 8 * gl + 8 * L * c, vec, E - 8 * gl - 8 * L * c, v + 8 * c);
+}
+
+// Loss and gradient coefficients from the column sums: thread i of the CTA calls with every e it owns.
+__device__ __forceinline__ float block_sum(float x, float* s_red) {
+  __syncthreads();
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  float r = 0.0f;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) r += s_red[w];
+  return r;
+}
+__device__ __forceinline__ long long block_sum_int(long long x, long long* s_red) {
+  __syncthreads();
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  long long r = 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) r += s_red[w];
+  return r;
+}
+
+// P (column sums) and f (counts) of all experts in shared memory -> loss, c, counts.
+__device__ void finish(const float* s_p, const int32_t* s_f, int E, float* __restrict__ loss,
+                       float* __restrict__ coef, int32_t* __restrict__ freq_out) {
+  __shared__ float s_red[32];
+  __shared__ long long s_redi[32];
+  float p = 0.0f;
+  long long f = 0;
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    p += s_p[e];
+    f += s_f[e];
+  }
+  const float n = block_sum(p, s_red);
+  const long long F = block_sum_int(f, s_redi);
+  // no token counts, or no entry: the loss and the gradient are 0 (a NaN sum stays NaN)
+  const float inv_n = n == 0.0f ? 0.0f : 1.0f / n;
+  const float inv_f = F == 0 ? 0.0f : 1.0f / static_cast<float>(F);
+  float l = 0.0f;
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    l += (s_p[e] * inv_n) * (static_cast<float>(s_f[e]) * inv_f);
+    coef[e] = static_cast<float>(static_cast<long long>(s_f[e]) * E - F) * inv_f * inv_n;
+    if (freq_out) freq_out[e] = s_f[e];
+  }
+  l = block_sum(l, s_red);
+  if (threadIdx.x == 0) *loss = l * static_cast<float>(E);
+}
+
+// Dynamic shared memory: column sums [kSlThreads / max(L, 32)][E] (one copy per warp, or one), counts [E].
+template <typename InT, int L, int C>
+__global__ void __launch_bounds__(kSlThreads)
+    switch_loss_kernel(const InT* __restrict__ logits, int T, int E, int vec, const uint8_t* __restrict__ mask,
+                       const int32_t* __restrict__ idx, int K, const int32_t* __restrict__ freq_in,
+                       float* __restrict__ part_p, int32_t* __restrict__ part_f, float* __restrict__ loss,
+                       float* __restrict__ coef, int32_t* __restrict__ freq_out, int* __restrict__ err) {
+  constexpr int kGroups = kSlThreads / L;               // rows in flight per CTA
+  constexpr int kCopies = L < 32 ? kSlThreads / 32 : kGroups;
+  extern __shared__ float s_dyn[];
+  __shared__ float s_red[8];
+  float* s_p = s_dyn;
+  int32_t* s_f = reinterpret_cast<int32_t*>(s_dyn + static_cast<size_t>(kCopies) * E);
+  const int gl = threadIdx.x % L, grp = threadIdx.x / L;
+  if (idx)
+    for (int e = threadIdx.x; e < E; e += kSlThreads) s_f[e] = 0;
+  float acc[8 * C];
+#pragma unroll
+  for (int i = 0; i < 8 * C; ++i) acc[i] = 0.0f;
+  // every group takes the same number of rows, so that the shuffles and barriers below are uniform
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T;
+       r0 += static_cast<long long>(gridDim.x) * kGroups) {
+    const long long r = r0 + grp;
+    const bool on = r < T && (!mask || mask[r]);
+    float v[8 * C];
+    if (on) {
+      load_row<InT, L, C>(logits + r * E, E, vec, gl, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) v[i] = 0.0f;
+    }
+    const float inv = softmax_row<L, C>(v, s_red);
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
+    }
+  }
+  // rows of one warp first (lanes that hold the same columns), then the warps through shared memory
+  if constexpr (L < 32) {
+#pragma unroll
+    for (int o = 16; o >= L; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+  }
+  if (L >= 32 || (threadIdx.x & 31) < L) {
+    float* dst = s_p + static_cast<size_t>(L < 32 ? threadIdx.x / 32 : grp) * E;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int e = 8 * gl + 8 * L * c + j;
+        if (e < E) dst[e] = acc[8 * c + j];
+      }
+  }
+  __syncthreads();
+  if (idx) {
+    const int n = T * K;
+    for (int i = blockIdx.x * kSlThreads + threadIdx.x; i < n; i += gridDim.x * kSlThreads) {
+      if (mask && !mask[i / K]) continue;
+      const int e = idx[i];
+      if (e >= 0 && e < E)
+        atomicAdd(&s_f[e], 1);
+      else
+        atomicCAS(err, 0, kErrBadExpert);
+    }
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < E; e += kSlThreads) {
+    float p = s_p[e];
+    for (int k = 1; k < kCopies; ++k) p += s_p[static_cast<size_t>(k) * E + e];
+    if (gridDim.x == 1) {
+      s_p[e] = p;
+      if (!idx) s_f[e] = freq_in[e];
+    } else {
+      part_p[static_cast<size_t>(blockIdx.x) * E + e] = p;
+      if (idx) part_f[static_cast<size_t>(blockIdx.x) * E + e] = s_f[e];
+    }
+  }
+  if (gridDim.x == 1) {
+    __syncthreads();
+    finish(s_p, s_f, E, loss, coef, freq_out);
+  }
+}
+
+// The CTAs' sums, `slices` groups of threads each adding every slices-th part, then the groups in order.
+constexpr int kFinThreads = 1024;
+constexpr int kFinSlots = 4096;  // slices * E <= kFinSlots
+
+__global__ void __launch_bounds__(kFinThreads)
+    switch_loss_finish_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_f, int parts, int E,
+                              int slices, const int32_t* __restrict__ freq_in, float* __restrict__ loss,
+                              float* __restrict__ coef, int32_t* __restrict__ freq_out) {
+  __shared__ float s_p[kFinSlots];
+  __shared__ int32_t s_f[kFinSlots];
+  for (int i = threadIdx.x; i < slices * E; i += kFinThreads) {
+    const int sl = i / E, e = i - sl * E;
+    float p = 0.0f;
+    int f = 0;
+#pragma unroll 8
+    for (int k = sl; k < parts; k += slices) {
+      p += part_p[static_cast<size_t>(k) * E + e];
+      if (part_f) f += part_f[static_cast<size_t>(k) * E + e];
+    }
+    s_p[i] = p;
+    s_f[i] = f;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kFinThreads) {
+    float p = s_p[e];
+    int f = s_f[e];
+    for (int sl = 1; sl < slices; ++sl) {
+      p += s_p[sl * E + e];
+      f += s_f[sl * E + e];
+    }
+    s_p[e] = p;
+    s_f[e] = part_f ? f : freq_in[e];
+  }
+  __syncthreads();
+  finish(s_p, s_f, E, loss, coef, freq_out);
+}
+
+template <typename InT, int L, int C>
+__global__ void __launch_bounds__(kSlThreads)
+    switch_loss_bwd_kernel(const InT* __restrict__ logits, int T, int E, int vec, const uint8_t* __restrict__ mask,
+                           const float* __restrict__ coef, const float* __restrict__ dloss,
+                           InT* __restrict__ dlogits) {
+  constexpr int kGroups = kSlThreads / L;
+  __shared__ float s_red[8];
+  const int gl = threadIdx.x % L, grp = threadIdx.x / L;
+  const float g = *dloss;
+  float c[8 * C];
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = 8 * gl + 8 * L * k + j;
+      c[8 * k + j] = e < E ? coef[e] : 0.0f;
+    }
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T;
+       r0 += static_cast<long long>(gridDim.x) * kGroups) {
+    const long long r = r0 + grp;
+    const bool on = r < T && (!mask || mask[r]);
+    float v[8 * C];
+    if (on) {
+      load_row<InT, L, C>(logits + r * E, E, vec, gl, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) v[i] = 0.0f;
+    }
+    const float inv = softmax_row<L, C>(v, s_red);
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * C; ++i) dot = fmaf(v[i], c[i], dot);
+    dot = row_reduce<L, false>(dot, s_red) * inv;
+    if (r >= T) continue;
+    // a token that does not count gets a gradient of exactly 0, whatever its logits hold
+#pragma unroll
+    for (int i = 0; i < 8 * C; ++i) v[i] = on ? g * (v[i] * inv * (c[i] - dot)) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+      store8<InT>(dlogits + r * E + 8 * gl + 8 * L * k, vec, E - 8 * gl - 8 * L * k, v + 8 * k);
+  }
+}
+
+// Aligned accesses of a row's 8-value pieces: 8, 4 or 1 values at a time.
+int vec_of(const void* p, int E, int esize) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  if (esize == 4) return E % 4 == 0 && a % 16 == 0 ? 4 : 1;
+  if (E % 8 == 0 && a % 16 == 0) return 8;
+  return E % 4 == 0 && a % 8 == 0 ? 4 : 1;
+}
+
+struct SlArgs {
+  const void* logits;
+  int T, E;
+  const uint8_t* mask;
+  const int32_t* idx;
+  int K;
+  const int32_t* freq_in;
+  float* part_p;
+  int32_t* part_f;
+  float* loss;
+  float* coef;
+  int32_t* freq_out;
+  int* err;
+  const float* dloss;
+  void* dlogits;
+  int grid;
+};
+
+template <typename InT, int L, int C>
+cudaError_t launch_lc(const SlArgs& a, bool bwd, cudaStream_t st) {
+  const InT* x = static_cast<const InT*>(a.logits);
+  if (bwd) {
+    int vec = vec_of(a.logits, a.E, sizeof(InT));
+    const int v2 = vec_of(a.dlogits, a.E, sizeof(InT));
+    vec = v2 < vec ? v2 : vec;
+    switch_loss_bwd_kernel<InT, L, C><<<a.grid, kSlThreads, 0, st>>>(x, a.T, a.E, vec, a.mask, a.coef, a.dloss,
+                                                                      static_cast<InT*>(a.dlogits));
+    return cudaGetLastError();
+  }
+  constexpr int kCopies = L < 32 ? kSlThreads / 32 : kSlThreads / L;
+  const int smem = (kCopies + 1) * a.E * 4;
+  switch_loss_kernel<InT, L, C><<<a.grid, kSlThreads, smem, st>>>(
+      x, a.T, a.E, vec_of(a.logits, a.E, sizeof(InT)), a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss,
+      a.coef, a.freq_out, a.err);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.grid == 1) return e;
+  const int slices = a.E >= kFinThreads ? 1 : kFinThreads / a.E;
+  switch_loss_finish_kernel<<<1, kFinThreads, 0, st>>>(a.part_p, a.idx ? a.part_f : nullptr, a.grid, a.E,
+                                                       slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef,
+                                                       a.freq_out);
+  return cudaGetLastError();
+}
+
+// Lanes per row: as many as hold the row at 8 values each, up to a warp; wider rows take 16 or 32
+// values a lane, and beyond 1024 experts a whole CTA shares the row.
+int lanes_of(int E) { return E <= 32 ? 4 : E <= 64 ? 8 : E <= 128 ? 16 : E <= 1024 ? 32 : kSlThreads; }
+
+template <typename InT>
+cudaError_t launch_t(const SlArgs& a, bool bwd, cudaStream_t st) {
+  if (a.E <= 32) return launch_lc<InT, 4, 1>(a, bwd, st);
+  if (a.E <= 64) return launch_lc<InT, 8, 1>(a, bwd, st);
+  if (a.E <= 128) return launch_lc<InT, 16, 1>(a, bwd, st);
+  if (a.E <= 256) return launch_lc<InT, 32, 1>(a, bwd, st);
+  if (a.E <= 512) return launch_lc<InT, 32, 2>(a, bwd, st);
+  if (a.E <= 1024) return launch_lc<InT, 32, 4>(a, bwd, st);
+  return launch_lc<InT, kSlThreads, 2>(a, bwd, st);
+}
+
+cudaError_t launch(const SlArgs& a, int dtype, bool bwd, cudaStream_t st) {
+  switch (dtype) {
+    case kDtypeBF16:
+      return launch_t<__nv_bfloat16>(a, bwd, st);
+    case kDtypeF16:
+      return launch_t<__half>(a, bwd, st);
+    default:
+      return launch_t<float>(a, bwd, st);
+  }
+}
+
+}  // namespace
+
+int switch_loss_parts(int T, int E) {
+  const int rows = 8 * (kSlThreads / lanes_of(E));  // at least 8 steps a CTA
+  const int want = ceil_div(T, rows);
+  return want < 1 ? 1 : want > 2 * 148 ? 2 * 148 : want;
+}
+
+cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,
+                               int K, const int32_t* freq_in, float* part_p, int32_t* part_f, float* loss,
+                               float* coef, int32_t* freq_out, int* err, cudaStream_t st) {
+  SlArgs a{logits, T, E, mask, idx, K, freq_in, part_p, part_f, loss, coef, freq_out, err, nullptr, nullptr,
+           switch_loss_parts(T, E)};
+  return launch(a, dtype, false, st);
+}
+
+cudaError_t launch_switch_loss_bwd(const void* logits, int dtype, int T, int E, const uint8_t* mask,
+                                   const float* coef, const float* dloss, void* dlogits, cudaStream_t st) {
+  if (T == 0) return cudaSuccess;
+  SlArgs a{};
+  a.logits = logits;
+  a.T = T;
+  a.E = E;
+  a.mask = mask;
+  a.coef = const_cast<float*>(coef);
+  a.dloss = dloss;
+  a.dlogits = dlogits;
+  const int rows = kSlThreads / lanes_of(E);
+  const int want = ceil_div(T, rows);
+  a.grid = want > 8 * 148 ? 8 * 148 : want;
+  return launch(a, dtype, true, st);
+}
+
+}  // namespace smb

@@ -720,3 +720,217 @@ int sm_moe_general_forward(const void* x, int T, int H, int I, int E, int TK, co
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------------------------
+// balance loss and 4-bit expert weights
+
+namespace {
+
+struct SlWs {
+  float* part_p;
+  int32_t* part_f;
+  int32_t* err;
+};
+
+SlWs carve_switch_loss(Carve& c, int T, int E) {
+  SlWs w;
+  const size_t n = static_cast<size_t>(switch_loss_parts(T, E)) * E;
+  w.part_p = c.take<float>(n);
+  w.part_f = c.take<int32_t>(n);
+  w.err = c.take<int32_t>(1);
+  return w;
+}
+
+int check_switch_loss_args(int T, int E, int dtype) {
+  if (T < 0) return fail(SM_EINVAL, "T must be >= 0 (got %d)", T);
+  if (E < 1 || E > 4096) return fail(SM_EINVAL, "E must be in [1, 4096] (got %d)", E);
+  if (dtype < 0 || dtype > 2) return fail(SM_EINVAL, "unknown logits dtype %d", dtype);
+  return SM_OK;
+}
+
+struct Int4Ws {
+  RouteWs route;
+  int32_t* off;
+  int32_t* s_scatter;
+  int32_t* s_rev;
+  int32_t* x_gather;
+  int32_t* tok_off;
+  void* a;
+  float* y;
+  int32_t* err;
+};
+
+Int4Ws carve_int4(Carve& c, int T, int n_entries, int H, int I, int E) {
+  Int4Ws w;
+  w.route = carve_route(c, T, n_entries, E);
+  w.off = c.take<int32_t>(E + 1);
+  w.s_scatter = c.take<int32_t>(n_entries);
+  w.s_rev = c.take<int32_t>(n_entries);
+  w.x_gather = c.take<int32_t>(n_entries);
+  w.tok_off = c.take<int32_t>(static_cast<size_t>(T) + 1);
+  w.a = c.take<uint16_t>(static_cast<size_t>(n_entries) * I);
+  w.y = c.take<float>(static_cast<size_t>(n_entries) * H);
+  w.err = c.take<int32_t>(1);
+  return w;
+}
+
+int check_int4_weight(int E, int N, int K, int group, int concat) {
+  if (E < 1 || E > 4096) return fail(SM_EINVAL, "E must be in [1, 4096] (got %d)", E);
+  if (N < 8 || N % 8 || K < 8 || K % 8)
+    return fail(SM_ENOTSUP, "4-bit expert weights need N and K positive multiples of 8 (got N=%d K=%d)", N, K);
+  if (group != 32 && group != 64 && group != 128) return fail(SM_ENOTSUP, "group must be 32, 64 or 128 (got %d)", group);
+  if (concat && N % 16) return fail(SM_EINVAL, "concatenated GLU weight needs N = 2I with I %% 8 == 0 (got N=%d)", N);
+  return SM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sm_switch_loss_workspace(int T, int E) {
+  Carve c{nullptr, 0};
+  carve_switch_loss(c, T > 0 ? T : 0, E > 0 ? E : 1);
+  return c.used + 256;
+}
+
+int sm_switch_loss(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                   const int32_t* topk_indices, int K, const int32_t* expert_frequency, float* loss, float* coef,
+                   int32_t* expert_frequency_out, void* workspace, size_t workspace_bytes, int32_t* err,
+                   void* stream) {
+  int rc = check_switch_loss_args(T, E, dtype);
+  if (rc) return rc;
+  if ((K > 0) == (expert_frequency != nullptr) || (K <= 0 && topk_indices))
+    return fail(SM_EINVAL, "give either the top-k indices (and K >= 1) or the expert counts (and K = 0)");
+  if (K < 0 || static_cast<long long>(T) * K > (1ll << 30))
+    return fail(SM_EINVAL, "need K >= 0 and T*K <= 2^30 (T=%d K=%d)", T, K);
+  if ((T > 0 && !router_logits) || !loss || !coef || !workspace) return fail(SM_EINVAL, "null pointer");
+  if (K > 0 && (!expert_frequency_out || (T > 0 && !topk_indices))) return fail(SM_EINVAL, "null pointer");
+  if (K > 0 && !topk_indices) topk_indices = expert_frequency_out;  // T = 0: nothing is read
+  Carve c{static_cast<uint8_t*>(workspace), workspace_bytes};
+  SlWs w = carve_switch_loss(c, T, E);
+  if (!c.ok) return fail(SM_EINVAL, "workspace too small (%zu < %zu)", workspace_bytes, c.used);
+  return cuda_status(launch_switch_loss(router_logits, dtype, T, E, token_mask, topk_indices, K, expert_frequency,
+                                        w.part_p, w.part_f, loss, coef, expert_frequency_out, err ? err : w.err,
+                                        static_cast<cudaStream_t>(stream)),
+                     "switch_loss");
+}
+
+int sm_switch_loss_bwd(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                       const float* coef, const float* dloss, void* dlogits, void* stream) {
+  int rc = check_switch_loss_args(T, E, dtype);
+  if (rc) return rc;
+  if (T > 0 && (!router_logits || !coef || !dloss || !dlogits)) return fail(SM_EINVAL, "null pointer");
+  return cuda_status(launch_switch_loss_bwd(router_logits, dtype, T, E, token_mask, coef, dloss, dlogits,
+                                            static_cast<cudaStream_t>(stream)),
+                     "switch_loss_bwd");
+}
+
+size_t sm_int4_weight_bytes(int E, int N, int K) {
+  return static_cast<size_t>(E) * int4_row_tiles(N) * int4_col_blocks(K) * 1024;
+}
+
+size_t sm_int4_scale_count(int E, int N, int K, int group) {
+  return static_cast<size_t>(E) * int4_row_tiles(N) * int4_col_blocks(K) * (128 / (group > 0 ? group : 128)) * 16;
+}
+
+int sm_weight_prep_int4(const void* w, int E, int N, int K, int group, int concat_glu, uint8_t* wq, void* scales,
+                        void* stream) {
+  int rc = check_int4_weight(E, N, K, group, concat_glu);
+  if (rc) return rc;
+  if (!w || !wq || !scales) return fail(SM_EINVAL, "null pointer");
+  if (!aligned16(w) || !aligned16(wq) || !aligned16(scales)) return fail(SM_EINVAL, "pointers must be 16-byte aligned");
+  return cuda_status(launch_weight_prep_int4(w, E, N, K, group, concat_glu, wq, scales,
+                                             static_cast<cudaStream_t>(stream)),
+                     "weight_prep_int4");
+}
+
+int sm_int4_expand(const uint8_t* wq, const void* scales, int E, int N, int K, int group, int concat_glu, void* w,
+                   void* stream) {
+  int rc = check_int4_weight(E, N, K, group, concat_glu);
+  if (rc) return rc;
+  if (!w || !wq || !scales) return fail(SM_EINVAL, "null pointer");
+  if (!aligned16(w) || !aligned16(wq) || !aligned16(scales)) return fail(SM_EINVAL, "pointers must be 16-byte aligned");
+  return cuda_status(launch_int4_expand(wq, scales, E, N, K, group, concat_glu, w, static_cast<cudaStream_t>(stream)),
+                     "int4_expand");
+}
+
+size_t sm_moe_int4_workspace_bytes(int T, int n_entries, int H, int I, int E) {
+  Carve c{nullptr, 0};
+  carve_int4(c, T, n_entries, H, I, E);
+  return c.used + 256;
+}
+
+int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_entries, const float* scores,
+                        const int32_t* token_indices, const int32_t* expert_indices, const uint8_t* w1q,
+                        const void* w1_scales, int w1_group, const uint8_t* w2q, const void* w2_scales, int w2_group,
+                        void* out, int32_t* expert_frequency, void* workspace, size_t workspace_bytes, int32_t* err,
+                        void* stream) {
+  if (T < 0 || n_entries < 0 || n_entries > (1 << 30))
+    return fail(SM_EINVAL, "need T >= 0 and 0 <= entries <= 2^30 (T=%d, entries=%d)", T, n_entries);
+  int rc = check_int4_weight(E, 2 * I, H, w1_group, 0);
+  if (rc) return rc;
+  rc = check_int4_weight(E, H, I, w2_group, 0);
+  if (rc) return rc;
+  if (K < 0 || (K > 0 && static_cast<long long>(T) * K != n_entries))
+    return fail(SM_EINVAL, "top-k arrays have T*K entries (T=%d K=%d, entries=%d)", T, K, n_entries);
+  if (!expert_frequency || (T > 0 && !out)) return fail(SM_EINVAL, "null pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0 || n_entries == 0) {
+    cudaError_t e0 = cudaMemsetAsync(expert_frequency, 0, sizeof(int32_t) * E, st);
+    if (e0 == cudaSuccess && T > 0) e0 = cudaMemsetAsync(out, 0, static_cast<size_t>(T) * H * 2, st);
+    return cuda_status(e0, "moe_int4_forward");
+  }
+  if (!x || !scores || !expert_indices || !w1q || !w1_scales || !w2q || !w2_scales || !workspace ||
+      (K == 0) != (token_indices != nullptr))
+    return fail(SM_EINVAL, "null pointer, or a token list beside top-k arrays");
+  if (!aligned16(x) || !aligned16(out) || !aligned16(w1q) || !aligned16(w2q) || !aligned16(w1_scales) ||
+      !aligned16(w2_scales) || !aligned16(workspace))
+    return fail(SM_EINVAL, "pointers must be 16-byte aligned");
+  Carve c{static_cast<uint8_t*>(workspace), workspace_bytes};
+  Int4Ws w = carve_int4(c, T, n_entries, H, I, E);
+  if (!c.ok) return fail(SM_EINVAL, "workspace too small (%zu < %zu)", workspace_bytes, c.used);
+  int32_t* errw = err ? err : w.err;
+  cudaError_t e = cudaSuccess;
+  if (!err) e = cudaMemsetAsync(w.err, 0, sizeof(int32_t), st);
+  const int per_tile = token_indices ? 1024 : kTileTokens * K;
+  const int n_tiles = token_indices ? route_tiles_general(n_entries) : route_tiles_tc(T);
+  if (e == cudaSuccess)
+    e = launch_route_hist(expert_indices, n_entries, per_tile, E, n_tiles, w.route.tile_counts, errw, st);
+  if (e == cudaSuccess)
+    e = launch_route_scan(w.route.tile_counts, n_tiles, E, n_entries, expert_frequency, w.off, w.route.off_pad,
+                          w.route.blk_expert, w.route.n_blocks, st);
+  if (e == cudaSuccess)
+    e = launch_route_scatter(expert_indices, token_indices, n_entries, K > 0 ? K : 1, per_tile, E, n_tiles,
+                             w.route.tile_counts, w.off, w.s_scatter, w.s_rev, w.x_gather, st);
+  if (e == cudaSuccess && token_indices) e = launch_token_offset(token_indices, T, n_entries, w.tok_off, st);
+  if (e == cudaSuccess) {
+    Int4Args p{};
+    p.x = x;
+    p.T = T;
+    p.H = H;
+    p.I = I;
+    p.E = E;
+    p.K = K;
+    p.experts = expert_indices;
+    p.scores = scores;
+    p.tok_off = token_indices ? w.tok_off : nullptr;
+    p.w1q = w1q;
+    p.w1s = w1_scales;
+    p.group1 = w1_group;
+    p.w2q = w2q;
+    p.w2s = w2_scales;
+    p.group2 = w2_group;
+    p.freq = expert_frequency;
+    p.off = w.off;
+    p.s_scatter = w.s_scatter;
+    p.x_gather = w.x_gather;
+    p.a = w.a;
+    p.y = w.y;
+    p.out = out;
+    p.err = errw;
+    e = launch_int4_experts(p, st);
+  }
+  return cuda_status(e, "moe_int4_forward");
+}
+
+}  // extern "C"

@@ -24,6 +24,7 @@ enum DevError : int {
   kErrBadExpert = 201,
   kErrBadReturnRow = 202,  // an up-projection row whose home rank / row lies outside the home buffers
   kErrBadCount = 203,  // expert parallel: an exchange count read on the device lies outside the buffers
+  kErrBadToken = 204,  // an explicit routing list names a token outside [0, T)
 };
 
 // A single wait never legitimately lasts more than a few milliseconds; 2 s means a bug.

@@ -79,6 +79,45 @@ cudaError_t launch_tq_pack(const void* src, int C, int src_padded, const int32_t
 cudaError_t launch_router_bwd(const void* logits, const float* scores, const int32_t* idx, const float* ds, int T,
                               int E, int K, int sot, int renorm, float* dlogits, cudaStream_t st);
 
+// router balance loss (csrc/balance.cu); parts = CTAs of the forward = rows of part_p / part_f [parts, E]
+int switch_loss_parts(int T, int E);
+cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,
+                               int K, const int32_t* freq_in, float* part_p, int32_t* part_f, float* loss,
+                               float* coef, int32_t* freq_out, int* err, cudaStream_t st);
+cudaError_t launch_switch_loss_bwd(const void* logits, int dtype, int T, int E, const uint8_t* mask,
+                                   const float* coef, const float* dloss, void* dlogits, cudaStream_t st);
+
+// 4-bit expert weights (csrc/int4.cu): 16-row tiles and 128-column blocks of a prepared [N, K] weight
+int int4_row_tiles(int N);
+int int4_col_blocks(int K);
+cudaError_t launch_weight_prep_int4(const void* w, int E, int N, int K, int group, int concat, uint8_t* wq, void* ws,
+                                    cudaStream_t st);
+cudaError_t launch_int4_expand(const uint8_t* wq, const void* ws, int E, int N, int K, int group, int concat, void* w,
+                               cudaStream_t st);
+struct Int4Args {
+  const void* x;  // bf16 [T, H]
+  int T, H, I, E, K;
+  const int32_t* experts;  // flat entries
+  const float* scores;
+  const int32_t* tok_off;  // explicit lists: entries [tok_off[t], tok_off[t + 1]) of token t; null: K a token
+  const uint8_t* w1q;
+  const void* w1s;
+  int group1;
+  const uint8_t* w2q;
+  const void* w2s;
+  int group2;
+  // routing plan: counts, offsets and the entries in expert order
+  const int32_t* freq;
+  const int32_t* off;
+  const int32_t* s_scatter;
+  const int32_t* x_gather;
+  void* a;   // bf16 [entries, I]
+  float* y;  // [entries, H]
+  void* out;
+  int* err;
+};
+cudaError_t launch_int4_experts(const Int4Args& p, cudaStream_t st);
+
 struct GemmArgs {
   // A: padded expert-major activations [rows, Kd] e4m3 + SF atoms [rows/128][ceil(Kd/512)][512]
   const uint8_t* a;

@@ -5,5 +5,5 @@ hand-written sm_100a kernels (libsonic_b200.so).  Drop-in import path: put ``son
 __version__ = "0.1.0+b200"
 
 from .enums import ActivationType, KernelBackendMoE
-from .functional import moe_general_routing_inputs, moe_TC_softmax_topk_layer
+from .functional import moe_general_routing_inputs, moe_TC_softmax_topk_layer, switch_load_balancing_loss
 from .moe import MoE

@@ -24,6 +24,7 @@ ERR_NAMES = {
     201: "expert index outside [0, E)",
     202: "up-projection row without a valid home row (home-down expert parallel)",
     203: "exchange count outside the expert-parallel buffers (device-side counts)",
+    204: "token index outside [0, T)",
 }
 
 _P = ctypes.c_void_p
@@ -116,6 +117,18 @@ SIGNATURES = {
     "sm_moe_down_combine": (
         _I,
         [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "sm_switch_loss_workspace": (_SZ, [_I, _I]),
+    "sm_switch_loss": (_I, [_P, _I, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _SZ, _P, _P]),
+    "sm_switch_loss_bwd": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "sm_int4_weight_bytes": (_SZ, [_I, _I, _I]),
+    "sm_int4_scale_count": (_SZ, [_I, _I, _I, _I]),
+    "sm_weight_prep_int4": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "sm_int4_expand": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P]),
+    "sm_moe_int4_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "sm_moe_int4_forward": (
+        _I,
+        [_P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _SZ, _P, _P],
     ),
 }
 

@@ -13,7 +13,9 @@ Weight-format contract (reference ``functional/__init__.py:560-566``): ``w1`` is
 ``[g0, u0, g1, u1, ...]`` or, with ``concat_layout=True``, ``[g0..g_{I-1}, u0..u_{I-1}]``;
 ``w2`` is the ``(H, I, E)`` view of ``c_proj.weight`` ``[E, H, I]``.  The bf16 weights are
 quantised to e4m3 with 128x128 UE8M0 block scales on first use and cached per weight version;
-already prepared :class:`~sonicmoe.ops.Fp8ExpertWeights` may be passed instead.
+already prepared :class:`~sonicmoe.ops.Fp8ExpertWeights` may be passed instead, or for inference
+:class:`~sonicmoe.ops.Int4ExpertWeights` (``prepare_int4_weights``: 4-bit codes with group scales, x
+kept in bf16; decoding is bound by the weights' bytes).
 
 Op boundary: as in the reference, the router top-k (``sonicmoe::_topk_fwd``,
 ``sonicmoe::_softmax_topk_fwd``, in ``forward.py``) and the routing metadata
@@ -43,7 +45,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..enums import ActivationType
-from ..ops import Fp8ExpertWeights
+from ..ops import Fp8ExpertWeights, Int4ExpertWeights
 from .forward import _topk_fwd, _topk_softmax_fwd  # noqa: F401  (registers the router ops)
 
 __all__ = [
@@ -52,7 +54,10 @@ __all__ = [
     "TC_topk_router_metadata_triton",
     "general_routing_router_metadata_triton",
     "prepare_fp8_weights",
+    "prepare_int4_weights",
+    "switch_load_balancing_loss",
     "Fp8ExpertWeights",
+    "Int4ExpertWeights",
 ]
 
 # Prepared FP8 weights, per tensor that owns the weight's storage (the root of its view chain):
@@ -111,6 +116,28 @@ def prepare_fp8_weights(w, concat_glu: bool = False, with_t: bool = False) -> Fp
         _WEIGHT_CACHE[key] = (ref, per_owner)
     per_owner[layout] = (state, prepared)  # only the newest version of each layout is kept
     return prepared
+
+
+def prepare_int4_weights(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False) -> Int4ExpertWeights:
+    """4-bit version, with a scale per ``group_size`` (32, 64 or 128) input columns, of an expert weight
+    given in the reference's (N, K, E) view.  Nothing is cached: the caller keeps the result."""
+    with torch.no_grad():
+        return ops.weight_prep_int4(_as_expert_major(w.detach()), group_size, concat_glu=concat_glu)
+
+
+def _int4_pair(w1, w2, concat_layout) -> bool:
+    """True for 4-bit expert weights (both must be, and w1 prepared for concat_layout)."""
+    if not (isinstance(w1, Int4ExpertWeights) or isinstance(w2, Int4ExpertWeights)):
+        return False
+    if not (isinstance(w1, Int4ExpertWeights) and isinstance(w2, Int4ExpertWeights)):
+        raise ValueError("w1 and w2 must both be 4-bit expert weights")
+    if w1.concat_glu != bool(concat_layout):
+        raise ValueError("prepared w1 layout does not match concat_layout")
+    return True
+
+
+def _prepared(w) -> bool:
+    return isinstance(w, (Fp8ExpertWeights, Int4ExpertWeights))
 
 
 def _check_common(b1, b2, activation_type):
@@ -253,6 +280,41 @@ def _(x, router_scores, token_indices, expert_indices, w1, w2, concat_layout):
     return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(w2.shape[-1], dtype=torch.int32)
 
 
+def _int4_tc(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
+             is_softmax_over_topk, norm_topk_probs):
+    scores, idx = ops.router_topk(router_logits, K, is_softmax_over_topk, norm_topk_probs)
+    return ops.moe_int4_forward(x, scores, idx, Int4ExpertWeights(w1q, w1_scales, tuple(w1_shape), w1_group, False),
+                                Int4ExpertWeights(w2q, w2_scales, tuple(w2_shape), w2_group, False))
+
+
+@torch.library.custom_op("sonicmoe::int4_moe_tc_forward", mutates_args=())
+def _int4_moe_tc_forward(
+    x: torch.Tensor,
+    router_logits: torch.Tensor,
+    w1q: torch.Tensor,
+    w1_scales: torch.Tensor,
+    w2q: torch.Tensor,
+    w2_scales: torch.Tensor,
+    w1_shape: list[int],
+    w2_shape: list[int],
+    w1_group: int,
+    w2_group: int,
+    K: int,
+    is_softmax_over_topk: bool,
+    norm_topk_probs: bool,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``moe_TC_softmax_topk_layer`` after the router GEMM on 4-bit expert weights (the prepared
+    ``Int4ExpertWeights`` taken apart): (o [T, H] bf16, expert_frequency [E] int32)."""
+    return _int4_tc(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
+                    is_softmax_over_topk, norm_topk_probs)
+
+
+@_int4_moe_tc_forward.register_fake
+def _(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
+      is_softmax_over_topk, norm_topk_probs):
+    return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(router_logits.shape[1], dtype=torch.int32)
+
+
 class _FP8MoEGeneralFunction(torch.autograd.Function):
     """Training forward + FP8 backward of the layer over explicit routing lists
     (``moe_general_routing_inputs``, reference functional/__init__.py:571-652 with its autograd
@@ -330,12 +392,25 @@ def moe_TC_softmax_topk_layer(
     if norm_topk_probs and is_softmax_over_topk:
         raise ValueError("`norm_topk_prob` only works with softmax-then-topk")
     training = _wants_training(is_inference_mode_enabled, x, router_w, w1, w2)
-    if training and (fused_router or isinstance(w1, Fp8ExpertWeights) or isinstance(w2, Fp8ExpertWeights)):
+    if training and (fused_router or _prepared(w1) or _prepared(w2)):
         raise NotImplementedError("the FP8 backward covers bf16 weights with the F.linear router "
                                   "(no fused_router or prepared weights)")
+    int4 = _int4_pair(w1, w2, concat_layout)
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
     x = x.contiguous()
+    if int4:
+        if fused_router:
+            router_logits, scores, idx = ops.router_fused(x, router_w.to(x.dtype).contiguous(), K,
+                                                          is_softmax_over_topk, norm_topk_probs)
+            o, expert_frequency = ops.moe_int4_forward(x, scores, idx, w1, w2)
+            return o, router_logits, expert_frequency
+        router_logits = F.linear(x, router_w.to(x.dtype))
+        layer = _int4_moe_tc_forward if torch.compiler.is_compiling() else _int4_tc
+        o, expert_frequency = layer(x, router_logits.contiguous(), w1.q, w1.scales, w2.q, w2.scales, list(w1.shape),
+                                    list(w2.shape), w1.group_size, w2.group_size, K, is_softmax_over_topk,
+                                    norm_topk_probs)
+        return o, router_logits, expert_frequency
     if training:
         router_logits = F.linear(x, router_w.to(x.dtype))
         o, expert_frequency = _FP8MoEFunction.apply(x, router_logits, w1, w2, K, is_softmax_over_topk,
@@ -393,8 +468,9 @@ def moe_general_routing_inputs(
     """
     _check_common(b1, b2, activation_type)
     training = _wants_training(is_inference_mode_enabled, x, router_scores, w1, w2)
-    if training and (isinstance(w1, Fp8ExpertWeights) or isinstance(w2, Fp8ExpertWeights)):
+    if training and (_prepared(w1) or _prepared(w2)):
         raise NotImplementedError("the FP8 backward covers bf16 weights (no prepared weights)")
+    int4 = _int4_pair(w1, w2, concat_layout)
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
     x = x.contiguous()
@@ -402,6 +478,8 @@ def moe_general_routing_inputs(
         router_scores = router_scores.float()
     args = (x, router_scores.contiguous(), token_indices.to(torch.int32).contiguous(),
             expert_indices.to(torch.int32).contiguous())
+    if int4:
+        return ops.moe_int4_general_forward(*args, w1, w2)
     if training:
         return _FP8MoEGeneralFunction.apply(*args, w1, w2, concat_layout)
     if isinstance(w1, Fp8ExpertWeights) or isinstance(w2, Fp8ExpertWeights):
@@ -409,6 +487,104 @@ def moe_general_routing_inputs(
         w2q = prepare_fp8_weights(w2, concat_glu=False)
         return ops.moe_general_forward(*args, w1q, w2q)
     return _fp8_moe_general_forward(*args, w1, w2, concat_layout)
+
+
+class _SwitchLossFunction(torch.autograd.Function):
+    """Balance loss with its gradient for the router logits; the counts carry none."""
+
+    @staticmethod
+    def forward(ctx, router_logits, expert_frequency, topk_indices, token_mask):
+        loss, freq, coef = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
+        ctx.save_for_backward(router_logits, coef, token_mask)
+        ctx.mark_non_differentiable(freq)
+        return loss, freq
+
+    @staticmethod
+    def backward(ctx, dloss, _dfreq):
+        router_logits, coef, token_mask = ctx.saved_tensors
+        if torch.is_grad_enabled():  # create_graph: the same formula in operations autograd can follow
+            p = F.softmax(router_logits, dim=-1, dtype=torch.float32)
+            if token_mask is not None:
+                p = p.where(token_mask[:, None] != 0, 0.0)
+            dl = dloss * p * (coef - (p * coef).sum(-1, keepdim=True))
+            return dl.to(router_logits.dtype), None, None, None
+        return ops.switch_loss_bwd(router_logits, coef, dloss.to(torch.float32), token_mask), None, None, None
+
+
+@torch.library.custom_op("sonicmoe::switch_loss", mutates_args=())
+def _switch_loss_op(
+    router_logits: torch.Tensor,
+    expert_frequency: torch.Tensor | None,
+    topk_indices: torch.Tensor | None,
+    token_mask: torch.Tensor | None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``ops.switch_loss`` for traced callers: (loss fp32 [], counts int32 [E], coef fp32 [E])."""
+    return ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
+
+
+@_switch_loss_op.register_fake
+def _(router_logits, expert_frequency, topk_indices, token_mask):
+    E = router_logits.shape[1]
+    return (router_logits.new_empty((), dtype=torch.float32), router_logits.new_empty(E, dtype=torch.int32),
+            router_logits.new_empty(E, dtype=torch.float32))
+
+
+@torch.library.custom_op("sonicmoe::switch_loss_bwd", mutates_args=())
+def _switch_loss_bwd_op(router_logits: torch.Tensor, coef: torch.Tensor, dloss: torch.Tensor,
+                        token_mask: torch.Tensor | None) -> torch.Tensor:
+    return ops.switch_loss_bwd(router_logits, coef, dloss, token_mask)
+
+
+@_switch_loss_bwd_op.register_fake
+def _(router_logits, coef, dloss, token_mask):
+    return torch.empty_like(router_logits)
+
+
+def _switch_loss_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], output[2], inputs[3])
+
+
+def _switch_loss_backward(ctx, dloss, _dfreq, _dcoef):
+    router_logits, coef, token_mask = ctx.saved_tensors
+    return _switch_loss_bwd_op(router_logits, coef, dloss.to(torch.float32), token_mask), None, None, None
+
+
+_switch_loss_op.register_autograd(_switch_loss_backward, setup_context=_switch_loss_setup)
+
+
+def switch_load_balancing_loss(
+    router_logits: torch.Tensor,
+    expert_frequency: torch.Tensor | None = None,
+    topk_indices: torch.Tensor | None = None,
+    token_mask: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Switch load-balancing loss of the router (the formula of reference moe.py:263-276) and the experts'
+    counts: (loss fp32 [], expert_frequency int32 [E]), differentiable with respect to router_logits.
+
+        p = softmax(router_logits), loss = E * sum_e (sum_t p[t, e] / sum p) (f_e / sum f)
+
+    Args:
+        router_logits: [T, E], bf16, fp16 or fp32.
+        expert_frequency: [E] counts f, as ``moe_TC_softmax_topk_layer`` returns them; or
+        topk_indices: [T, K] expert ids, as ``ops.router_topk`` returns them, which are counted here.
+            Exactly one of the two is given; neither gets a gradient.
+        token_mask: [T] bool, optional: tokens that are False (padding) take no part in the
+            probabilities, in the counts made from topk_indices, or in the gradient.
+
+    The loss is 0 when no token or no entry counts.  The same inputs give the same bits.
+    """
+    router_logits = router_logits.contiguous()
+    if expert_frequency is not None:
+        expert_frequency = expert_frequency.to(torch.int32).contiguous()
+    if topk_indices is not None:
+        topk_indices = topk_indices.to(torch.int32).contiguous()
+    if token_mask is not None:
+        token_mask = token_mask.contiguous()
+    if torch.compiler.is_compiling():
+        loss, freq, _ = _switch_loss_op(router_logits, expert_frequency, topk_indices, token_mask)
+    else:
+        loss, freq = _SwitchLossFunction.apply(router_logits, expert_frequency, topk_indices, token_mask)
+    return loss, freq
 
 
 @torch.library.custom_op(

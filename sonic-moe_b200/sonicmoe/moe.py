@@ -8,10 +8,9 @@ this package has no eager-torch or scattermoe execution path, and asking for one
 """
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
 from .enums import ActivationType, KernelBackendMoE, is_glu
-from .functional import moe_TC_softmax_topk_layer
+from .functional import moe_TC_softmax_topk_layer, prepare_int4_weights, switch_load_balancing_loss
 
 
 class Experts(nn.Module):
@@ -40,6 +39,8 @@ class Experts(nn.Module):
 
 
 class MoE(nn.Module):
+    _int4_experts = None  # set by use_int4_experts
+
     def __init__(
         self,
         num_experts: int,
@@ -75,6 +76,19 @@ class MoE(nn.Module):
         # current torch stream at call time, so nothing is queried at construction
         self.stream_id = None
 
+    def use_int4_experts(self, group_size: int | None = 128) -> "MoE":
+        """Run inference forwards on 4-bit copies of the present expert weights, with a scale per
+        ``group_size`` (32, 64 or 128) input columns; None goes back to the FP8 engine.
+
+        The copies are made here, on the weights' device, and kept: after changing the weights or moving the
+        module, call it again.  A forward that needs gradients raises NotImplementedError meanwhile."""
+        if group_size is None:
+            self._int4_experts = None
+        else:
+            self._int4_experts = tuple(prepare_int4_weights(w.weight.permute(1, 2, 0), group_size)
+                                       for w in (self.c_fc, self.c_proj))
+        return self
+
     def forward(
         self,
         hidden_states: torch.Tensor,
@@ -85,14 +99,18 @@ class MoE(nn.Module):
             raise NotImplementedError(
                 f"backend {kernel_backend_moe} is not provided by the B200 engine; use KernelBackendMoE.sonicmoe"
             )
+        if self._int4_experts is not None:
+            w1, w2 = self._int4_experts
+        else:
+            w1, w2 = self.c_fc.weight.permute(1, 2, 0), self.c_proj.weight.permute(1, 2, 0)
         original_shape = hidden_states.shape
         hidden_states = hidden_states.view(-1, self.hidden_size)
         hidden_states, router_logits, expert_frequency = moe_TC_softmax_topk_layer(
             hidden_states,
             self.router.weight,
-            self.c_fc.weight.permute(1, 2, 0),
+            w1,
             self.c_fc.bias,
-            self.c_proj.weight.permute(1, 2, 0),
+            w2,
             self.c_proj.bias,
             self.top_k,
             self.stream_id,
@@ -103,18 +121,5 @@ class MoE(nn.Module):
         if is_inference_mode:
             aux_loss = None
         else:
-            aux_loss = self._compute_switch_loss(
-                logits=router_logits,
-                probs=F.softmax(router_logits, dim=-1, dtype=torch.float32),
-                expert_frequency=expert_frequency,
-            )
+            aux_loss, _ = switch_load_balancing_loss(router_logits, expert_frequency)
         return hidden_states, aux_loss
-
-    def _compute_switch_loss(self, logits, probs, expert_frequency):
-        """Switch load-balancing loss (reference moe.py:263-276), plain torch on the device."""
-        logits = logits.view(-1, logits.size(-1))
-        probs = probs.view(-1, probs.size(-1))
-        num_experts = logits.size(1)
-        acc_probs = probs.sum(0)
-        expert_frequency = expert_frequency.float()
-        return num_experts * (F.normalize(acc_probs, p=1, dim=0) * F.normalize(expert_frequency, p=1, dim=0)).sum()

@@ -588,3 +588,198 @@ def moe_backward(dout: torch.Tensor, x: torch.Tensor, router_logits: torch.Tenso
     ds = ds.view(T, K)
     dlogits = router_bwd(router_logits, scores, idx, ds, softmax_over_topk, norm_topk_probs)
     return dx, dlogits, dw1, dw2, ds
+
+
+# ---------------------------------------------------------------------------------------------
+# router balance loss and 4-bit expert weights
+
+
+def _same_device(first: torch.Tensor, **others):
+    """Every other tensor (None: absent) lies on the first one's device."""
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {first.device}")
+
+
+def _call_on(device: torch.device, name: str, *args):
+    """Enqueue an entry point on the current stream of the tensors' device, whichever device is current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        nat.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            nat.call(name, *args, stream)
+
+
+def _check_mask(token_mask, T: int):
+    if token_mask is None:
+        return
+    _need(token_mask, "token_mask")
+    if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (T,):
+        raise ValueError(f"token_mask must be bool or uint8 [{T}], got {token_mask.dtype} {tuple(token_mask.shape)}")
+
+
+def _check_logits(router_logits: torch.Tensor):
+    _need(router_logits, "router_logits")
+    if router_logits.dim() != 2:
+        raise ValueError(f"router_logits must be [T, E], got {tuple(router_logits.shape)}")
+    if router_logits.dtype not in _LOGIT_DTYPES:
+        raise ValueError(f"unsupported logits dtype {router_logits.dtype}")
+
+
+def switch_loss(router_logits: torch.Tensor, expert_frequency: torch.Tensor = None, topk_indices: torch.Tensor = None,
+                token_mask: torch.Tensor = None, err: torch.Tensor = None):
+    """Switch balance loss of the router (reference moe.py:263-276) and the counts it used: (loss fp32 [],
+    expert_frequency int32 [E], coef fp32 [E] for ``switch_loss_bwd``).
+
+    router_logits [T, E]; exactly one of expert_frequency (int32 [E], counts as given) and topk_indices
+    (int32 [T, K], counted here).  token_mask [T] (bool or uint8): tokens with 0, such as padding, count
+    neither in the loss nor in the counts made here.  The sums have a fixed order."""
+    _check_logits(router_logits)
+    T, E = router_logits.shape
+    if (expert_frequency is None) == (topk_indices is None):
+        raise ValueError("give either expert_frequency or topk_indices")
+    _same_device(router_logits, expert_frequency=expert_frequency, topk_indices=topk_indices, token_mask=token_mask,
+                 err=err)
+    _check_mask(token_mask, T)
+    K = 0
+    if topk_indices is not None:
+        _need(topk_indices, "topk_indices", torch.int32)
+        if topk_indices.dim() != 2 or topk_indices.shape[0] != T:
+            raise ValueError(f"topk_indices must be [{T}, K], got {tuple(topk_indices.shape)}")
+        K = topk_indices.shape[1]
+    else:
+        _need(expert_frequency, "expert_frequency", torch.int32)
+        if tuple(expert_frequency.shape) != (E,):
+            raise ValueError(f"expert_frequency must be [{E}], got {tuple(expert_frequency.shape)}")
+    dev = router_logits.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    coef = torch.empty(E, dtype=torch.float32, device=dev)
+    freq = torch.empty(E, dtype=torch.int32, device=dev)
+    ws = _workspace(nat.load().sm_switch_loss_workspace(T, E), dev)
+    _call_on(dev, "sm_switch_loss", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E, _ptr(token_mask),
+             _ptr(topk_indices), K, _ptr(expert_frequency), _ptr(loss), _ptr(coef), _ptr(freq), _ptr(ws), ws.numel(),
+             _ptr(err))
+    return loss, freq, coef
+
+
+def switch_loss_bwd(router_logits: torch.Tensor, coef: torch.Tensor, dloss: torch.Tensor,
+                    token_mask: torch.Tensor = None):
+    """Gradient of ``switch_loss`` with respect to the logits [T, E] (their dtype), times dloss (fp32 [])."""
+    _check_logits(router_logits)
+    T, E = router_logits.shape
+    _same_device(router_logits, coef=coef, dloss=dloss, token_mask=token_mask)
+    _need(coef, "coef", torch.float32)
+    _need(dloss, "dloss", torch.float32)
+    if tuple(coef.shape) != (E,) or dloss.numel() != 1:
+        raise ValueError(f"coef must be [{E}] and dloss a single value")
+    _check_mask(token_mask, T)
+    dl = torch.empty_like(router_logits)
+    _call_on(router_logits.device, "sm_switch_loss_bwd", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E,
+             _ptr(token_mask), _ptr(coef), _ptr(dloss), _ptr(dl))
+    return dl
+
+
+@dataclass
+class Int4ExpertWeights:
+    """4-bit expert weights with group scales, as produced by ``weight_prep_int4``.
+
+    ``q``: the codes, ``scales``: bf16, both in the library's own order; ``shape``: (E, N, K) of the
+    weight; ``group_size``: input columns that share a scale; ``concat_glu``: the caller's w1 was
+    concatenated [gate; up].
+    """
+
+    q: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple
+    group_size: int
+    concat_glu: bool
+
+
+def weight_prep_int4(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False) -> Int4ExpertWeights:
+    """Quantise expert weights [E, N, K] (bf16) to codes in [-7, 7] with a scale per ``group_size`` (32,
+    64 or 128) input columns: the smallest number of 5 significant bits that is >= amax / 7."""
+    if w.dim() != 3:
+        raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
+    if w.dtype != torch.bfloat16:
+        w = w.to(torch.bfloat16)
+    w = w.contiguous()
+    _need(w, "w", torch.bfloat16)
+    E, N, K = w.shape
+    lib = nat.load()
+    q = torch.empty(lib.sm_int4_weight_bytes(E, N, K), dtype=torch.uint8, device=w.device)
+    scales = torch.empty(lib.sm_int4_scale_count(E, N, K, group_size), dtype=torch.bfloat16, device=w.device)
+    _call_on(w.device, "sm_weight_prep_int4", _ptr(w), E, N, K, group_size, int(concat_glu), _ptr(q), _ptr(scales))
+    return Int4ExpertWeights(q, scales, (E, N, K), group_size, bool(concat_glu))
+
+
+def int4_expand(w: Int4ExpertWeights) -> torch.Tensor:
+    """The bf16 weights [E, N, K] that a prepared 4-bit weight stands for, exactly (for a long prompt:
+    ``weight_prep`` of them gives the FP8 engine's weights)."""
+    E, N, K = w.shape
+    out = torch.empty(E, N, K, dtype=torch.bfloat16, device=w.q.device)
+    _call_on(out.device, "sm_int4_expand", _ptr(w.q), _ptr(w.scales), E, N, K, w.group_size, int(w.concat_glu),
+             _ptr(out))
+    return out
+
+
+def _moe_int4(x, scores, token_indices, expert_indices, n_entries, K, w1, w2, out, expert_frequency, err):
+    _need(x, "x", torch.bfloat16)
+    _need(scores, "scores", torch.float32)
+    _need(expert_indices, "expert indices", torch.int32)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, H], got {tuple(x.shape)}")
+    T, H = x.shape
+    E, N2, H1 = w1.shape
+    E2, H2, I = w2.shape
+    if H1 != H or H2 != H or N2 != 2 * I or E2 != E:
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w1 {w1.shape}, w2 {w2.shape}")
+    if w2.concat_glu:
+        raise ValueError("w2 was prepared with concat_glu")
+    _same_device(x, scores=scores, token_indices=token_indices, expert_indices=expert_indices, w1=w1.q, w2=w2.q,
+                 out=out, expert_frequency=expert_frequency, err=err)
+    dev = x.device
+    if out is None:
+        out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)
+    else:
+        _need(out, "out", torch.bfloat16)
+        if tuple(out.shape) != (T, H):
+            raise ValueError(f"out must be [{T}, {H}]")
+    if expert_frequency is None:
+        expert_frequency = torch.empty(E, dtype=torch.int32, device=dev)
+    else:
+        _need(expert_frequency, "expert_frequency", torch.int32)
+        if tuple(expert_frequency.shape) != (E,):
+            raise ValueError(f"expert_frequency must be [{E}]")
+    ws = _workspace(nat.load().sm_moe_int4_workspace_bytes(T, n_entries, H, I, E), dev)
+    _call_on(dev, "sm_moe_int4_forward", _ptr(x), T, H, I, E, K, n_entries, _ptr(scores), _ptr(token_indices),
+             _ptr(expert_indices), _ptr(w1.q), _ptr(w1.scales), w1.group_size, _ptr(w2.q), _ptr(w2.scales),
+             w2.group_size, _ptr(out), _ptr(expert_frequency), _ptr(ws), ws.numel(), _ptr(err))
+    return out, expert_frequency
+
+
+def moe_int4_forward(x: torch.Tensor, topk_scores: torch.Tensor, topk_indices: torch.Tensor, w1: Int4ExpertWeights,
+                     w2: Int4ExpertWeights, out: torch.Tensor = None, expert_frequency: torch.Tensor = None,
+                     err: torch.Tensor = None):
+    """The experts' part of the layer on 4-bit weights, for routed tokens: (out [T, H] bf16,
+    expert_frequency [E] int32) from x [T, H] bf16, topk_scores fp32 and topk_indices int32 [T, K].
+
+    x is not quantised; the products are accumulated in fp32, the intermediate is rounded to bf16 and
+    the output once, and a token's experts are added in a fixed order."""
+    if topk_indices.dim() != 2 or topk_indices.shape[0] != x.shape[0] or topk_scores.shape != topk_indices.shape:
+        raise ValueError(f"topk_scores and topk_indices must be [T, K] for T = {x.shape[0]}, got "
+                         f"{tuple(topk_scores.shape)} and {tuple(topk_indices.shape)}")
+    return _moe_int4(x, topk_scores, None, topk_indices, topk_indices.numel(), topk_indices.shape[1], w1, w2, out,
+                     expert_frequency, err)
+
+
+def moe_int4_general_forward(x: torch.Tensor, router_scores: torch.Tensor, token_indices: torch.Tensor,
+                             expert_indices: torch.Tensor, w1: Int4ExpertWeights, w2: Int4ExpertWeights,
+                             out: torch.Tensor = None, expert_frequency: torch.Tensor = None,
+                             err: torch.Tensor = None):
+    """``moe_int4_forward`` for explicit (token, expert, score) entries, token_indices sorted ascending."""
+    _need(token_indices, "token_indices", torch.int32)
+    n = expert_indices.numel()
+    if router_scores.numel() != n or token_indices.numel() != n:
+        raise ValueError(f"routing lists of {token_indices.numel()}, {n} and {router_scores.numel()} entries")
+    return _moe_int4(x, router_scores, token_indices, expert_indices, n, 0, w1, w2, out, expert_frequency, err)
