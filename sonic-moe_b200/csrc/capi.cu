@@ -889,13 +889,40 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   Carve c{static_cast<uint8_t*>(workspace), workspace_bytes};
   Int4Ws w = carve_int4(c, T, n_entries, H, I, E);
   if (!c.ok) return fail(SM_EINVAL, "workspace too small (%zu < %zu)", workspace_bytes, c.used);
-  int32_t* errw = err ? err : w.err;
+  Int4Args p{};
+  p.x = x;
+  p.T = T;
+  p.H = H;
+  p.I = I;
+  p.E = E;
+  p.K = K;
+  p.experts = expert_indices;
+  p.tokens = token_indices;
+  p.n_entries = n_entries;
+  p.scores = scores;
+  p.tok_off = token_indices ? w.tok_off : nullptr;
+  p.w1q = w1q;
+  p.w1s = w1_scales;
+  p.group1 = w1_group;
+  p.w2q = w2q;
+  p.w2s = w2_scales;
+  p.group2 = w2_group;
+  p.freq = expert_frequency;
+  p.off = w.off;
+  p.s_scatter = w.s_scatter;
+  p.x_gather = w.x_gather;
+  p.a = w.a;
+  p.y = w.y;
+  p.out = out;
+  p.err = err;
+  if (int4_small(T, n_entries)) return cuda_status(launch_int4_small(p, st), "moe_int4_forward");
+  p.err = err ? err : w.err;
   cudaError_t e = cudaSuccess;
   if (!err) e = cudaMemsetAsync(w.err, 0, sizeof(int32_t), st);
   const int per_tile = token_indices ? 1024 : kTileTokens * K;
   const int n_tiles = token_indices ? route_tiles_general(n_entries) : route_tiles_tc(T);
   if (e == cudaSuccess)
-    e = launch_route_hist(expert_indices, n_entries, per_tile, E, n_tiles, w.route.tile_counts, errw, st);
+    e = launch_route_hist(expert_indices, n_entries, per_tile, E, n_tiles, w.route.tile_counts, p.err, st);
   if (e == cudaSuccess)
     e = launch_route_scan(w.route.tile_counts, n_tiles, E, n_entries, expert_frequency, w.off, w.route.off_pad,
                           w.route.blk_expert, w.route.n_blocks, st);
@@ -903,33 +930,7 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
     e = launch_route_scatter(expert_indices, token_indices, n_entries, K > 0 ? K : 1, per_tile, E, n_tiles,
                              w.route.tile_counts, w.off, w.s_scatter, w.s_rev, w.x_gather, st);
   if (e == cudaSuccess && token_indices) e = launch_token_offset(token_indices, T, n_entries, w.tok_off, st);
-  if (e == cudaSuccess) {
-    Int4Args p{};
-    p.x = x;
-    p.T = T;
-    p.H = H;
-    p.I = I;
-    p.E = E;
-    p.K = K;
-    p.experts = expert_indices;
-    p.scores = scores;
-    p.tok_off = token_indices ? w.tok_off : nullptr;
-    p.w1q = w1q;
-    p.w1s = w1_scales;
-    p.group1 = w1_group;
-    p.w2q = w2q;
-    p.w2s = w2_scales;
-    p.group2 = w2_group;
-    p.freq = expert_frequency;
-    p.off = w.off;
-    p.s_scatter = w.s_scatter;
-    p.x_gather = w.x_gather;
-    p.a = w.a;
-    p.y = w.y;
-    p.out = out;
-    p.err = errw;
-    e = launch_int4_experts(p, st);
-  }
+  if (e == cudaSuccess) e = launch_int4_experts(p, st);
   return cuda_status(e, "moe_int4_forward");
 }
 

@@ -15,9 +15,11 @@
 // of column 2 i, nibble i + 4 that of column 2 i + 1, so (word >> 4 i) & 0x000F000F is a pair of
 // neighbours in the halves of a register.  A column block's order inside the product does not matter
 // as long as x is read the same way: lane l reads 8 consecutive values of x (16 bytes) for each word
-// pair, and two m16n8k16 products consume them.  Scales are [tile][group][16] bf16, row g at 2 g, row
-// g + 8 at 2 g + 1.  A GLU weight's prepared row 2 j is gate row j and 2 j + 1 up row j (the
+// pair, and two m16n8k16 products consume them.  The scales of a block are [8][groups][2] bf16: for
+// g < 8 and each group of the block, rows g and g + 8 (one load of 4, 8 or 16 bytes a lane).  A GLU weight's prepared row 2 j is gate row j and 2 j + 1 up row j (the
 // interleaved order; a concatenated w1 is re-ordered when it is prepared).
+#include <type_traits>
+
 #include "common.cuh"
 #include "sonic_internal.h"
 
@@ -90,7 +92,8 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
     const int h = c >> 3, blk = (c >> 2) & 1, t = c & 3;
     s_word[warp][h * 128 + (4 * (r & 7) + t) * 4 + 2 * blk + (r >> 3)] = word;
     if (c % lanes_per_group == 0)
-      ws[((et * k_blocks + kb) * gpb + c / lanes_per_group) * 16 + 2 * (r & 7) + (r >> 3)] = __float2bfloat16_rn(s);
+      ws[(et * k_blocks + kb) * gpb * 16 + ((r & 7) * gpb + c / lanes_per_group) * 2 + (r >> 3)] =
+          __float2bfloat16_rn(s);
   }
   __syncwarp();
   uint4* dst = reinterpret_cast<uint4*>(wq + (et * k_blocks + kb) * 1024);
@@ -121,7 +124,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
     const int h = c >> 3, blk = (c >> 2) & 1, t = c & 3;
     const uint32_t word = words[h * 128 + (4 * (r & 7) + t) * 4 + 2 * blk + (r >> 3)];
     const float s = __bfloat162float(
-        ws[((et * k_blocks + kb) * gpb + c / lanes_per_group) * 16 + 2 * (r & 7) + (r >> 3)]);
+        ws[(et * k_blocks + kb) * gpb * 16 + ((r & 7) * gpb + c / lanes_per_group) * 2 + (r >> 3)]);
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -135,10 +138,25 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
 // ---------------------------------------------------------------------------------------------
 // products
 
+// The constants come from registers the compiler cannot look into: with two immediates it would spend two
+// instructions instead of one on the and-or.
+struct Int4Magic {
+  uint32_t mask, base;
+  __device__ __forceinline__ Int4Magic() {
+    asm volatile("mov.u32 %0, 0x000F000F;" : "=r"(mask));
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(base));
+  }
+};
+__device__ __forceinline__ uint32_t int4_pair_raw(const Int4Magic& c, uint32_t w, int i) {  // 128 + n
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "r"(c.mask), "r"(c.base));  // (a & b) | c
+  return r;
+}
+
 // Codes of word `w`, pair i (columns 2 i, 2 i + 1), as two bf16: 0x4300 is 128, whose last mantissa bit
 // is worth 1, so 0x4300 | n is 128 + n, and subtracting 136 leaves q = n - 8 exactly.
-__device__ __forceinline__ uint32_t int4_pair(uint32_t w, int i) {
-  const uint32_t u = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+__device__ __forceinline__ uint32_t int4_pair(const Int4Magic& c, uint32_t w, int i) {
+  const uint32_t u = int4_pair_raw(c, w, i);
   const uint32_t off = 0x43084308u;
   __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<uint32_t*>(&r);
@@ -152,6 +170,15 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint3
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// d = a b + c
+__device__ __forceinline__ void mma_bf16_16816_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+
 constexpr int kMvWarps = 8;
 constexpr int kMvThreads = 32 * kMvWarps;
 
@@ -162,6 +189,7 @@ __device__ __forceinline__ void mv_tile(const uint8_t* __restrict__ wq, const __
                                         int K, int b0, int b1, const __nv_bfloat16* const (&xrow)[NT],
                                         float (&acc)[NT][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const Int4Magic magic;
   for (int b = b0; b < b1; ++b) {
     uint4 q[2];
     q[0] = __ldg(reinterpret_cast<const uint4*>(wq + static_cast<size_t>(b) * 1024) + lane);
@@ -180,8 +208,8 @@ __device__ __forceinline__ void mv_tile(const uint8_t* __restrict__ wq, const __
       uint32_t a[4], c[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        a[i] = int4_pair(lo, i);
-        c[i] = int4_pair(hi, i);
+        a[i] = int4_pair(magic, lo, i);
+        c[i] = int4_pair(magic, hi, i);
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -191,8 +219,8 @@ __device__ __forceinline__ void mv_tile(const uint8_t* __restrict__ wq, const __
         mma_bf16_16816(part[j], a[2], c[2], a[3], c[3], xv.z, xv.w);
       }
       if (((s + 1) * 32) % group == 0) {  // end of a group: its sums times the rows' scales
-        const uint32_t s2 = __ldg(reinterpret_cast<const uint32_t*>(
-                                      sc + (static_cast<size_t>(b) * gpb + (s * 32) / group) * 16) + g);
+        const uint32_t s2 = __ldg(reinterpret_cast<const uint32_t*>(sc + static_cast<size_t>(b) * gpb * 16) +
+                                  g * gpb + (s * 32) / group);
         const float slo = __uint_as_float(s2 << 16), shi = __uint_as_float(s2 & 0xFFFF0000u);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -307,6 +335,588 @@ __global__ void __launch_bounds__(kMvThreads) mv_kernel(const MvArgs p) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few tokens.  Two launches: the up projection and the down projection with the sum over a token's
+// experts.  Both read each weight of an active expert once and are bound by those bytes, so what counts
+// is how many loads are in flight:
+//   - every warp streams row tiles of its own (MT x 16 rows) through a ring of kDepth column blocks in
+//     shared memory, filled by 16-byte asynchronous copies ahead of the products, across the end of one
+//     tile and the start of the next; a lane reads back only what it copied itself, so the ring needs no
+//     barrier;
+//   - there is no routing pass: every CTA makes the list of active experts and their entries itself from
+//     the (few) expert ids while its first loads could not be issued anyway;
+//   - the down kernel starts while the up kernel drains (programmatic dependent launch) and has its first
+//     weights in registers before it waits for the intermediate.
+// The m16n8k16 tensor core product takes 8 tokens as its 8 columns; with one token 7/8 of its work is
+// thrown away, but it still keeps up with the memory, which the plain FMA units would not beyond 2 tokens.
+
+constexpr int kSmMaxEntries = 1024;
+
+// Active experts (slots, ascending) of the entries and their flat entries, slot s owning
+// list[beg[s]] .. list[beg[s + 1]).  The order inside a slot of up to `chunk` entries does not matter: an
+// entry's values do not depend on the column it has in a product.  Beyond that it decides which entries
+// share a pass, whose code differs with their number, so the lists are then made in entry order.
+struct SmallPlan {
+  uint16_t act[kSmMaxEntries];
+  uint16_t beg[kSmMaxEntries + 2];
+  uint16_t list[kSmMaxEntries];
+  int32_t scan[2][kMvWarps];
+};
+
+__device__ __forceinline__ int small_plan(const int32_t* __restrict__ experts, int n, int E, int chunk, int32_t* cnt,
+                                          SmallPlan& p, int32_t* freq_out, int* err) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (freq_out)
+    for (int e = tid; e < E; e += kMvThreads) freq_out[e] = 0;
+  if (n <= 32) {  // one warp finds equal experts by matching; slots in the order of first appearance
+    __syncthreads();  // freq_out is zero
+    if (warp == 0) {
+      int e = lane < n ? experts[lane] : -1;
+      const bool ok = e >= 0 && e < E;
+      if (lane < n && !ok && freq_out && err) atomicCAS(err, 0, kErrBadExpert);
+      const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
+      const uint32_t below = (1u << lane) - 1u;
+      const bool first = ok && (same & below) == 0;
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      const int c = first ? __popc(same) : 0;
+      int inc = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const int beg = __shfl_sync(0xffffffffu, inc - c, ok ? __ffs(same) - 1 : 0);
+      if (first) {
+        const int s = __popc(firsts & below);
+        p.act[s] = static_cast<uint16_t>(e);
+        p.beg[s] = static_cast<uint16_t>(beg);
+        if (freq_out) freq_out[e] = c;
+      }
+      if (ok) p.list[beg + __popc(same & below)] = static_cast<uint16_t>(lane);
+      if (lane == 31) {
+        p.beg[__popc(firsts)] = static_cast<uint16_t>(inc);
+        p.scan[0][0] = __popc(firsts);
+      }
+    }
+    __syncthreads();
+    return p.scan[0][0];
+  }
+  for (int e = tid; e < E; e += kMvThreads) cnt[e] = 0;
+  __syncthreads();
+  for (int f = tid; f < n; f += kMvThreads) {
+    const int e = experts[f];
+    if (e >= 0 && e < E)
+      atomicAdd(&cnt[e], 1);
+    else if (freq_out && err)
+      atomicCAS(err, 0, kErrBadExpert);
+  }
+  __syncthreads();
+  const int per = (E + kMvThreads - 1) / kMvThreads;
+  const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
+  int a = 0, c = 0;
+  bool large = false;
+  for (int e = e0; e < e1; ++e) {
+    const int v = cnt[e];
+    a += v > 0;
+    c += v;
+    large |= v > chunk;
+    if (freq_out) freq_out[e] = v;
+  }
+  int ia = a, ic = c;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int ya = __shfl_up_sync(0xffffffffu, ia, o), yc = __shfl_up_sync(0xffffffffu, ic, o);
+    if (lane >= o) {
+      ia += ya;
+      ic += yc;
+    }
+  }
+  if (lane == 31) {
+    p.scan[0][warp] = ia;
+    p.scan[1][warp] = ic;
+  }
+  __syncthreads();
+  ia -= a;
+  ic -= c;
+  int slots = 0;
+#pragma unroll
+  for (int w = 0; w < kMvWarps; ++w) {
+    const int sa = p.scan[0][w], sc = p.scan[1][w];
+    if (w < warp) {
+      ia += sa;
+      ic += sc;
+    }
+    slots += sa;
+  }
+  for (int e = e0; e < e1; ++e) {
+    const int v = cnt[e];
+    if (v == 0) continue;
+    p.act[ia] = static_cast<uint16_t>(e);
+    p.beg[ia] = static_cast<uint16_t>(ic);
+    cnt[e] = ic;  // becomes the next free place of e's list
+    ++ia;
+    ic += v;
+  }
+  if (tid == kMvThreads - 1) p.beg[slots] = static_cast<uint16_t>(ic);
+  if (__syncthreads_or(large)) {
+    if (warp == 0) {
+      for (int f0 = 0; f0 < n; f0 += 32) {
+        int e = f0 + lane < n ? experts[f0 + lane] : -1;
+        if (e < 0 || e >= E) e = -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const int at = e >= 0 ? cnt[e] + __popc(same & ((1u << lane) - 1u)) : 0;
+        __syncwarp();
+        if (e >= 0) {
+          p.list[at] = static_cast<uint16_t>(f0 + lane);
+          if ((same >> lane) == 1u) cnt[e] = at + 1;  // the last of its kind
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    for (int f = tid; f < n; f += kMvThreads) {
+      const int e = experts[f];
+      if (e >= 0 && e < E) p.list[atomicAdd(&cnt[e], 1)] = static_cast<uint16_t>(f);
+    }
+  }
+  __syncthreads();
+  return slots;
+}
+
+struct SmallArgs {
+  const uint8_t* wq;
+  const __nv_bfloat16* ws;
+  int N, K, n_tiles, k_blocks;  // prepared rows N, input columns K
+  const int32_t* experts;
+  const int32_t* tokens;  // explicit lists, else null: token f / topk
+  int n_entries, topk, T, E;
+  const __nv_bfloat16* x;  // up: tokens [T, K]; down: the intermediate [entries, K]
+  const float* scores;
+  __nv_bfloat16* a;    // up output [entries, N / 2]
+  __nv_bfloat16* out;  // down output [T, N]
+  int32_t* freq;
+  int ksplit;  // parts of the columns of a tile, one warp each
+  int* err;
+};
+
+// The intermediate is written by the grid this one overlaps with: not through the read-only path.
+__device__ __forceinline__ uint4 ld_plain(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A warp's ring: kDepth stages of one column block of MT row tiles, lane l's 16-byte piece h of tile m at
+// (2 m + h) * 512 + 16 l, then its scales (GPB words) at MT * 1024 + m * 128 GPB + 4 GPB l.
+template <int MT>
+constexpr int kDepth = MT == 1 ? 6 : 4;
+template <int MT, int GPB>
+constexpr int kStage = MT * (1024 + 128 * GPB);
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int kBytes>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+// src: the lane's piece of the block in the first tile's codes, sc: its scales; the second tile's lie
+// tile2 blocks further on.
+template <int MT, int GPB>
+__device__ __forceinline__ void fill_stage(uint32_t stage, const uint8_t* src, const __nv_bfloat16* sc, int tile2) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint8_t* q = src + static_cast<size_t>(m * tile2) * 1024;
+    const __nv_bfloat16* s = sc + static_cast<size_t>(m * tile2) * (GPB * 16);
+    cp_async16(stage + 1024 * m + 16 * lane, q);
+    cp_async16(stage + 1024 * m + 512 + 16 * lane, q + 512);
+    const uint32_t sd = stage + 1024 * MT + 128 * GPB * m + 4 * GPB * lane;
+    if constexpr (GPB == 4)
+      cp_async16(sd, s);
+    else
+      cp_async_small<4 * GPB>(sd, s);
+  }
+}
+
+// Values 8 t .. 8 t + 7 of the 32-column pieces of block b of a token's row; whole: the block lies inside K.
+template <bool kUp>
+__device__ __forceinline__ uint4 load_x(const __nv_bfloat16* xrow, int b, int s, int K, bool whole) {
+  const int k = b * 128 + 32 * s + 8 * (threadIdx.x & 3);
+  if (!whole && k >= K) return make_uint4(0, 0, 0, 0);
+  return kUp ? __ldg(reinterpret_cast<const uint4*>(xrow + k)) : ld_plain(xrow + k);
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+// One stage's products.  With few tokens (NT <= 2) the instructions per weight count: a group's sums are
+// scaled, in fp32, and the offset of the codes (128 + n stands for n - 8) is taken from the sums too, which
+// start at -136 times the sum of x, itself a product with a constant.  With more tokens the codes lose
+// their offset and are scaled (both exact), which leaves the sums of all groups in one accumulator.
+template <int MT, int NT, int GPB, bool kUp>
+__device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage, int b, int K, bool whole, const __nv_bfloat16* const* xrow,
+                                          const uint4* xv, float (*acc)[MT][4]) {
+  constexpr bool kSums = NT <= 2;
+  constexpr uint32_t kMinus136 = 0xC308C308u;
+  const int lane = threadIdx.x & 31;
+  float part[kSums ? NT : 1][MT][4];
+  uint4 q[MT];
+  uint32_t s2[MT][GPB];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const uint32_t a = stage + 1024 * MT + 128 * GPB * m + 4 * GPB * lane;
+    if constexpr (GPB == 4) {
+      const uint4 v = lds128(a);
+      s2[m][0] = v.x;
+      s2[m][1] = v.y;
+      s2[m][2] = v.z;
+      s2[m][3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < GPB; ++i) s2[m][i] = lds32(a + 4 * i);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {  // 32 columns each
+    const bool first = s % (4 / GPB) == 0, last = (s + 1) % (4 / GPB) == 0;
+    uint32_t lo[MT][4], hi[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (s % 2 == 0) q[m] = lds128(stage + 1024 * m + 256 * s + 16 * lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t wl = s & 1 ? q[m].z : q[m].x, wh = s & 1 ? q[m].w : q[m].y;
+        if constexpr (kSums) {
+          lo[m][i] = int4_pair_raw(magic, wl, i);
+          hi[m][i] = int4_pair_raw(magic, wh, i);
+        } else {
+          const uint32_t sw = s2[m][s / (4 / GPB)];
+          lo[m][i] = mul_bf16x2(int4_pair(magic, wl, i), __byte_perm(sw, 0, 0x1010));
+          hi[m][i] = mul_bf16x2(int4_pair(magic, wh, i), __byte_perm(sw, 0, 0x3232));
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const uint4 x = NT == 1 ? xv[s] : load_x<kUp>(xrow[j], b, s, K, whole);
+      if constexpr (!kSums) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_bf16_16816(acc[j][m], lo[m][0], hi[m][0], lo[m][1], hi[m][1], x.x, x.y);
+          mma_bf16_16816(acc[j][m], lo[m][2], hi[m][2], lo[m][3], hi[m][3], x.z, x.w);
+        }
+      } else {
+        float c[4];
+        mma_bf16_16816_c(c, kMinus136, kMinus136, kMinus136, kMinus136, x.x, x.y, 0.0f, 0.0f, 0.0f, 0.0f);
+        mma_bf16_16816(c, kMinus136, kMinus136, kMinus136, kMinus136, x.z, x.w);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          float(&d)[4] = part[j][m];
+          if (first) {
+            mma_bf16_16816_c(d, lo[m][0], hi[m][0], lo[m][1], hi[m][1], x.x, x.y, c[0], c[1], c[2], c[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] += c[i];
+            mma_bf16_16816(d, lo[m][0], hi[m][0], lo[m][1], hi[m][1], x.x, x.y);
+          }
+          mma_bf16_16816(d, lo[m][2], hi[m][2], lo[m][3], hi[m][3], x.z, x.w);
+          if (last) {
+            const uint32_t w = s2[m][s / (4 / GPB)];
+            const float slo = __uint_as_float(w << 16), shi = __uint_as_float(w & 0xFFFF0000u);
+            acc[j][m][0] = fmaf(slo, d[0], acc[j][m][0]);
+            acc[j][m][1] = fmaf(slo, d[1], acc[j][m][1]);
+            acc[j][m][2] = fmaf(shi, d[2], acc[j][m][2]);
+            acc[j][m][3] = fmaf(shi, d[3], acc[j][m][3]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// A warp's stream: items first, first + step, ... < count; decode(item) gives (slot, tile, columns part).
+// Tokens of an item come in chunks of 8 NT columns, each a pass over the item's blocks.  Calls
+// done(tile, part, beg, n, acc) after each pass; before_x() once after the first copies have been issued.
+template <int MT, int NT, int GPB, bool kUp, typename Decode, typename Done, typename BeforeX>
+__device__ __forceinline__ void stream_items(const SmallArgs& p, const SmallPlan& pl, uint32_t ring, int first,
+                                             int step, int count, Decode decode, BeforeX before_x, Done done) {
+  const int g = (threadIdx.x & 31) >> 2;
+  const Int4Magic magic;
+  // the copies' position: item, blocks left of this pass, passes' tokens left, addresses
+  int l_item = first, l_left = 0, l_tokens = 0, l_tile2 = 0;
+  const uint8_t* l_src = nullptr;
+  const __nv_bfloat16* l_sc = nullptr;
+  uint32_t l_stage = 0, u_stage = 0;
+  const int lane = threadIdx.x & 31;
+  auto bounds = [&](int part, int& b0, int& b1) {
+    b0 = part * p.k_blocks / p.ksplit;
+    b1 = (part + 1) * p.k_blocks / p.ksplit;
+  };
+  auto open = [&](bool next_pass) {
+    if (l_item >= count) return;
+    int slot, tile, part, b0, b1;
+    decode(l_item, slot, tile, part);
+    bounds(part, b0, b1);
+    if (!next_pass) l_tokens = pl.beg[slot + 1] - pl.beg[slot];
+    const size_t blk = (static_cast<size_t>(pl.act[slot]) * p.n_tiles + tile) * p.k_blocks + b0;
+    l_src = p.wq + blk * 1024 + 16 * lane;
+    l_sc = p.ws + blk * (GPB * 16) + (lane >> 2) * (GPB * 2);
+    // a second tile past the last one repeats the first; its results are dropped
+    l_tile2 = tile + 1 < p.n_tiles ? p.k_blocks : 0;
+    l_left = b1 - b0;
+  };
+  auto fill = [&] {
+    if (l_item < count) {
+      fill_stage<MT, GPB>(ring + l_stage * kStage<MT, GPB>, l_src, l_sc, l_tile2);
+      if (++l_stage == kDepth<MT>) l_stage = 0;
+      l_src += 1024;
+      l_sc += GPB * 16;
+      if (--l_left == 0) {
+        l_tokens -= 8 * NT;
+        const bool again = l_tokens > 0;
+        if (!again) l_item += step;
+        open(again);
+      }
+    }
+    cp_async_commit();
+  };
+  open(false);
+#pragma unroll
+  for (int d = 0; d < kDepth<MT> - 1; ++d) fill();
+  before_x();
+  for (int item = first; item < count; item += step) {
+    int slot, tile, part, b0, b1;
+    decode(item, slot, tile, part);
+    bounds(part, b0, b1);
+    const int end = pl.beg[slot + 1];
+    for (int beg = pl.beg[slot]; beg < end; beg += 8 * NT) {
+      const int n = min(end - beg, 8 * NT);
+      const __nv_bfloat16* xrow[NT];
+      float acc[NT][MT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        // columns without a token repeat another's row (any row serves); their results are dropped
+        const int f = pl.list[beg + min(8 * j + g, n - 1)];
+        if (kUp) {
+          int tok = p.tokens ? p.tokens[f] : f / p.topk;
+          if (tok < 0 || tok >= p.T) {
+            if (p.err) atomicCAS(p.err, 0, kErrBadToken);
+            tok = 0;  // the entry belongs to no token of the output: its results are not summed anywhere
+          }
+          xrow[j] = p.x + static_cast<size_t>(tok) * p.K;
+        } else {
+          xrow[j] = p.x + static_cast<size_t>(f) * p.K;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][m][i] = 0.0f;
+      }
+      auto pass = [&](auto nt) {
+        constexpr int kNt = decltype(nt)::value;
+        uint4 xv[4], x0[4];
+        auto load = [&](int b) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) xv[s] = load_x<kUp>(xrow[0], b, s, p.K, (b + 1) * 128 <= p.K);
+        };
+        if (kNt == 1) load(b0);
+        for (int b = b0; b < b1; ++b) {
+          if (kNt == 1) {  // the next block's x is under way during this one's products
+#pragma unroll
+            for (int s = 0; s < 4; ++s) x0[s] = xv[s];
+            if (b + 1 < b1) load(b + 1);
+          }
+          fill();  // the stage freed by the block before
+          cp_async_wait<kDepth<MT> - 1>();
+          use_stage<MT, kNt, GPB, kUp>(magic, ring + u_stage * kStage<MT, GPB>, b, p.K, (b + 1) * 128 <= p.K, xrow, x0, acc);
+          if (++u_stage == kDepth<MT>) u_stage = 0;
+        }
+      };
+      if (NT == 1 || n <= 8)
+        pass(std::integral_constant<int, 1>{});
+      else if (NT == 2 || n <= 16)
+        pass(std::integral_constant<int, (NT < 2 ? NT : 2)>{});
+      else
+        pass(std::integral_constant<int, NT>{});
+      done(tile, part, beg, n, acc);
+    }
+  }
+}
+
+__device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+// Up projection and SwiGLU: a persistent grid, item = (slot, MT row tiles).  With ksplit > 1 (few items)
+// adjacent warps of a CTA share a tile's columns and their sums meet in shared memory.
+template <int MT, int NT, int GPB>
+__global__ void __launch_bounds__(kMvThreads, 2) small_up_kernel(const SmallArgs p) {
+  extern __shared__ __align__(16) uint8_t s_dyn[];  // rings, counts [E]
+  __shared__ SmallPlan pl;
+  __shared__ float s_part[NT == 1 ? kMvWarps : 1][8][16 * MT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(s_dyn) + warp * kDepth<MT> * kStage<MT, GPB>;
+  int32_t* s_cnt = reinterpret_cast<int32_t*>(s_dyn + kMvWarps * kDepth<MT> * kStage<MT, GPB>);
+  pdl_launch();
+  const int slots = small_plan(p.experts, p.n_entries, p.E, 8 * NT, s_cnt, pl, blockIdx.x == 0 ? p.freq : nullptr, p.err);
+  const int tiles = (p.n_tiles + MT - 1) / MT, half = p.N / 2;
+  auto decode = [&](int item, int& slot, int& tile, int& part) {
+    part = item % p.ksplit;
+    const int i = item / p.ksplit;
+    slot = i / tiles;
+    tile = (i - slot * tiles) * MT;
+  };
+  const int count = slots * tiles * p.ksplit, step = gridDim.x * kMvWarps;
+  auto store = [&](int f, int col, float v) {
+    if (col < half) p.a[static_cast<size_t>(f) * half + col] = __float2bfloat16_rn(v);
+  };
+  if (NT > 1 || p.ksplit == 1) {
+    stream_items<MT, NT, GPB, true>(
+        p, pl, ring, blockIdx.x * kMvWarps + warp, step, count, decode, [] {},
+        [&](int tile, int, int beg, int n, float (&acc)[NT][MT][4]) {
+          // rows 2 r are gates, rows 2 r + 1 ups: lanes of even g finish row g's pair, their partners
+          // (lane ^ 4) row (g - 1) + 8's
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const bool odd = g & 1;
+              const float r0 = __shfl_xor_sync(0xffffffffu, odd ? acc[j][m][0] : acc[j][m][2], 4);
+              const float r1 = __shfl_xor_sync(0xffffffffu, odd ? acc[j][m][1] : acc[j][m][3], 4);
+              const float v0 = odd ? silu_mul(r0, acc[j][m][2]) : silu_mul(acc[j][m][0], r0);
+              const float v1 = odd ? silu_mul(r1, acc[j][m][3]) : silu_mul(acc[j][m][1], r1);
+              const int col = (tile + m) * 8 + (odd ? 4 : 0) + (g >> 1), i = 8 * j + 2 * t;
+              if (i < n) store(pl.list[beg + i], col, v0);
+              if (i + 1 < n) store(pl.list[beg + i + 1], col, v1);
+            }
+        });
+    return;
+  }
+  // every warp of the CTA takes the same number of rounds, one item (and one chunk of tokens) each
+  if constexpr (NT == 1)
+  for (int r = blockIdx.x * kMvWarps; r < count; r += step) {
+    stream_items<MT, NT, GPB, true>(
+        p, pl, ring, r + warp, count, min(count, r + kMvWarps), decode, [] {},
+        [&](int, int, int, int, float (&acc)[NT][MT][4]) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_part[warp][2 * t + (i & 1)][16 * m + g + 8 * (i >> 1)] = acc[0][m][i];
+        });
+    __syncthreads();
+    int slot, tile, part;
+    if (r + warp < count) {
+      decode(r + warp, slot, tile, part);
+      const int beg = pl.beg[slot], n = pl.beg[slot + 1] - beg;
+      for (int o = part * 32 + lane; o < n * 8 * MT; o += p.ksplit * 32) {
+        const int i = o / (8 * MT), row = o % (8 * MT);
+        float gate = 0.0f, up = 0.0f;
+        for (int k = 0; k < p.ksplit; ++k) {
+          gate += s_part[warp - part + k][i][2 * row];
+          up += s_part[warp - part + k][i][2 * row + 1];
+        }
+        store(pl.list[beg + i], tile * 8 + row, silu_mul(gate, up));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Down projection and the sum over each token's entries: a cluster owns MT row tiles for all active
+// experts, whose (slot, columns part) items its warps take in turn.  Every entry's result is written
+// once, into the first CTA's shared memory, and a token's entries are then added in entry order.
+template <int MT, int NT, int GPB>
+__global__ void __launch_bounds__(kMvThreads, 2) small_down_kernel(const SmallArgs p) {
+  // rings, counts [E], the results [ksplit][entries][16 MT] of the cluster
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  __shared__ SmallPlan pl;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(s_dyn) + warp * kDepth<MT> * kStage<MT, GPB>;
+  int32_t* s_cnt = reinterpret_cast<int32_t*>(s_dyn + kMvWarps * kDepth<MT> * kStage<MT, GPB>);
+  float* s_y = reinterpret_cast<float*>(s_cnt + p.E);
+  uint32_t rank, csize;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+  const int slots = small_plan(p.experts, p.n_entries, p.E, 8 * NT, s_cnt, pl, nullptr, p.err);
+  const int tile0 = static_cast<int>(blockIdx.x / csize) * MT;
+  uint32_t y0;  // the first CTA's results, as seen from this one
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(y0) : "r"(smem_u32(s_y)));
+  // the first CTA has started (its shared memory may be written)
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  stream_items<MT, NT, GPB, false>(
+      p, pl, ring, static_cast<int>(rank) * kMvWarps + warp, static_cast<int>(csize) * kMvWarps, slots * p.ksplit,
+      [&](int item, int& slot, int& tile, int& part) {
+        slot = item / p.ksplit;
+        part = item - slot * p.ksplit;
+        tile = tile0;
+      },
+      [] { pdl_wait(); },
+      [&](int, int part, int beg, int n, float (&acc)[NT][MT][4]) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int c = 8 * j + 2 * t + (i & 1);
+              if (c < n) {
+                const uint32_t at = (part * p.n_entries + pl.list[beg + c]) * (16 * MT) + 16 * m + g + 8 * (i >> 1);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(y0 + 4 * at), "f"(acc[j][m][i]) : "memory");
+              }
+            }
+      });
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank != 0) return;
+  for (int o = threadIdx.x; o < p.T * 16 * MT; o += kMvThreads) {
+    const int tok = o / (16 * MT), row = o % (16 * MT);
+    const int col = tile0 * 16 + row;
+    if (col >= p.N) continue;
+    int f0 = tok * p.topk, f1 = f0 + p.topk;
+    if (p.tokens) {  // sorted list: first entry of tok and of tok + 1
+      int lo = 0, hi = p.n_entries;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p.tokens[mid] < tok)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      f0 = lo;
+      f1 = f0;
+      while (f1 < p.n_entries && p.tokens[f1] == tok) ++f1;
+    }
+    float v = 0.0f;
+    for (int f = f0; f < f1; ++f) {
+      const int e = p.experts[f];
+      if (e < 0 || e >= p.E) continue;
+      float y = 0.0f;
+      for (int k = 0; k < p.ksplit; ++k) y += s_y[(k * p.n_entries + f) * (16 * MT) + row];
+      v = fmaf(p.scores[f], y, v);
+    }
+    p.out[static_cast<size_t>(tok) * p.N + col] = __float2bfloat16_rn(v);
+  }
+}
+
 // out[t] = sum of the rows y[f] of t's entries, f in [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]),
 // in entry order, rounded once.  Entries whose expert or token was rejected have no row.
 __global__ void __launch_bounds__(256)
@@ -351,6 +961,109 @@ cudaError_t launch_int4_expand(const uint8_t* wq, const void* ws, int E, int N, 
   int4_expand_kernel<<<static_cast<unsigned>((items + kPrepWarps - 1) / kPrepWarps), 32 * kPrepWarps, 0, st>>>(
       wq, static_cast<const __nv_bfloat16*>(ws), E, N, K, group, concat, nt, kb, static_cast<__nv_bfloat16*>(w));
   return cudaGetLastError();
+}
+
+namespace {
+
+template <int MT, int NT, int GPB>
+cudaError_t launch_small_up(SmallArgs p, cudaStream_t st) {
+  const int tiles = ceil_div(p.n_tiles, MT);
+  const int slots = p.E < p.n_entries ? p.E : p.n_entries;
+  auto kern = small_up_kernel<MT, NT, GPB>;
+  const int smem = kMvWarps * kDepth<MT> * kStage<MT, GPB> + p.E * 4;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  int occ = 0;
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kMvThreads, smem);
+  if (e != cudaSuccess) return e;
+  const long long most = static_cast<long long>(gemm_grid_sms()) * (occ > 0 ? occ : 1);
+  // few items: split their columns while that leaves one item a warp (an expert must fit one chunk)
+  p.ksplit = 1;
+  while (NT == 1 && p.n_entries <= 8 && p.ksplit < kMvWarps && 2 * p.ksplit <= p.k_blocks &&
+         static_cast<long long>(slots) * tiles * 2 * p.ksplit <= most * kMvWarps)
+    p.ksplit *= 2;
+  const long long ctas = ceil_div(static_cast<long long>(slots) * tiles * p.ksplit, kMvWarps);
+  kern<<<static_cast<unsigned>(ctas < most ? ctas : most), kMvThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <int MT, int NT, int GPB>
+cudaError_t launch_small_down(SmallArgs p, cudaStream_t st) {
+  const int tiles = ceil_div(p.n_tiles, MT);
+  const int slots = p.E < p.n_entries ? p.E : p.n_entries;
+  int cluster = 1;  // CTAs that share a row tile's experts, so that narrow outputs still fill the SMs
+  while (cluster < 8 && tiles * cluster < 200 && slots > 8 * cluster) cluster *= 2;
+  p.ksplit = 1;
+  while (slots * p.ksplit < kMvWarps * cluster && 2 * p.ksplit <= p.k_blocks && p.ksplit < kMvWarps &&
+         2 * p.ksplit * p.n_entries * 64 * MT <= 64 * 1024)
+    p.ksplit *= 2;
+  const int smem = kMvWarps * kDepth<MT> * kStage<MT, GPB> + p.E * 4 + p.ksplit * p.n_entries * 16 * MT * 4;
+  auto kern = small_down_kernel<MT, NT, GPB>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles * cluster);
+  cfg.blockDim = dim3(kMvThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<const SmallArgs>(p));
+}
+
+template <int MT, int NT>
+cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int group2, cudaStream_t st) {
+  cudaError_t e = group1 == 32   ? launch_small_up<MT, NT, 4>(u, st)
+                  : group1 == 64 ? launch_small_up<MT, NT, 2>(u, st)
+                                 : launch_small_up<MT, NT, 1>(u, st);
+  if (e != cudaSuccess) return e;
+  return group2 == 32   ? launch_small_down<MT, NT, 4>(d, st)
+         : group2 == 64 ? launch_small_down<MT, NT, 2>(d, st)
+                        : launch_small_down<MT, NT, 1>(d, st);
+}
+
+}  // namespace
+
+bool int4_small(int T, int n_entries) { return T <= 64 && n_entries <= kSmMaxEntries; }
+
+cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st) {
+  SmallArgs u{};
+  u.wq = p.w1q;
+  u.ws = static_cast<const __nv_bfloat16*>(p.w1s);
+  u.N = 2 * p.I;
+  u.K = p.H;
+  u.n_tiles = int4_row_tiles(u.N);
+  u.k_blocks = int4_col_blocks(u.K);
+  u.experts = p.experts;
+  u.tokens = p.tokens;
+  u.n_entries = p.n_entries;
+  u.topk = p.K;
+  u.T = p.T;
+  u.E = p.E;
+  u.x = static_cast<const __nv_bfloat16*>(p.x);
+  u.a = static_cast<__nv_bfloat16*>(p.a);
+  u.freq = p.freq;
+  u.err = p.err;
+  SmallArgs d = u;
+  d.wq = p.w2q;
+  d.ws = static_cast<const __nv_bfloat16*>(p.w2s);
+  d.N = p.H;
+  d.K = p.I;
+  d.n_tiles = int4_row_tiles(d.N);
+  d.k_blocks = int4_col_blocks(d.K);
+  d.x = u.a;
+  d.scores = p.scores;
+  d.out = static_cast<__nv_bfloat16*>(p.out);
+  if (p.T <= 8) return launch_small<2, 1>(u, p.group1, d, p.group2, st);
+  if (p.T <= 16) return launch_small<2, 2>(u, p.group1, d, p.group2, st);
+  return launch_small<2, 4>(u, p.group1, d, p.group2, st);
 }
 
 cudaError_t launch_int4_experts(const Int4Args& p, cudaStream_t st) {

@@ -98,6 +98,8 @@ struct Int4Args {
   const void* x;  // bf16 [T, H]
   int T, H, I, E, K;
   const int32_t* experts;  // flat entries
+  const int32_t* tokens;   // explicit lists: the entries' tokens, sorted; null: K entries a token
+  int n_entries;
   const float* scores;
   const int32_t* tok_off;  // explicit lists: entries [tok_off[t], tok_off[t + 1]) of token t; null: K a token
   const uint8_t* w1q;
@@ -107,7 +109,7 @@ struct Int4Args {
   const void* w2s;
   int group2;
   // routing plan: counts, offsets and the entries in expert order
-  const int32_t* freq;
+  int32_t* freq;
   const int32_t* off;
   const int32_t* s_scatter;
   const int32_t* x_gather;
@@ -117,6 +119,9 @@ struct Int4Args {
   int* err;
 };
 cudaError_t launch_int4_experts(const Int4Args& p, cudaStream_t st);
+// Few tokens: no routing plan (freq is written; off, s_scatter, x_gather, tok_off, y unused; err may be null).
+bool int4_small(int T, int n_entries);
+cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st);
 
 struct GemmArgs {
   // A: padded expert-major activations [rows, Kd] e4m3 + SF atoms [rows/128][ceil(Kd/512)][512]

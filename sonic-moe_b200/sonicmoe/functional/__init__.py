@@ -497,10 +497,13 @@ class _SwitchLossFunction(torch.autograd.Function):
         loss, freq, coef = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
         ctx.save_for_backward(router_logits, coef, token_mask)
         ctx.mark_non_differentiable(freq)
+        ctx.set_materialize_grads(False)
         return loss, freq
 
     @staticmethod
     def backward(ctx, dloss, _dfreq):
+        if dloss is None:
+            return None, None, None, None
         router_logits, coef, token_mask = ctx.saved_tensors
         if torch.is_grad_enabled():  # create_graph: the same formula in operations autograd can follow
             p = F.softmax(router_logits, dim=-1, dtype=torch.float32)
@@ -582,6 +585,8 @@ def switch_load_balancing_loss(
         token_mask = token_mask.contiguous()
     if torch.compiler.is_compiling():
         loss, freq, _ = _switch_loss_op(router_logits, expert_frequency, topk_indices, token_mask)
+    elif not (router_logits.requires_grad and torch.is_grad_enabled()):
+        loss, freq, _ = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
     else:
         loss, freq = _SwitchLossFunction.apply(router_logits, expert_frequency, topk_indices, token_mask)
     return loss, freq

@@ -654,8 +654,8 @@ def switch_loss(router_logits: torch.Tensor, expert_frequency: torch.Tensor = No
             raise ValueError(f"expert_frequency must be [{E}], got {tuple(expert_frequency.shape)}")
     dev = router_logits.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    coef = torch.empty(E, dtype=torch.float32, device=dev)
     freq = torch.empty(E, dtype=torch.int32, device=dev)
+    coef = torch.empty(E, dtype=torch.float32, device=dev)
     ws = _workspace(nat.load().sm_switch_loss_workspace(T, E), dev)
     _call_on(dev, "sm_switch_loss", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E, _ptr(token_mask),
              _ptr(topk_indices), K, _ptr(expert_frequency), _ptr(loss), _ptr(coef), _ptr(freq), _ptr(ws), ws.numel(),
