@@ -755,6 +755,7 @@ struct Int4Ws {
   int32_t* s_rev;
   int32_t* x_gather;
   int32_t* tok_off;
+  void* xs;
   void* a;
   float* y;
   int32_t* err;
@@ -768,8 +769,10 @@ Int4Ws carve_int4(Carve& c, int T, int n_entries, int H, int I, int E) {
   w.s_rev = c.take<int32_t>(n_entries);
   w.x_gather = c.take<int32_t>(n_entries);
   w.tok_off = c.take<int32_t>(static_cast<size_t>(T) + 1);
-  w.a = c.take<uint16_t>(static_cast<size_t>(n_entries) * I);
-  w.y = c.take<float>(static_cast<size_t>(n_entries) * H);
+  const bool small = int4_small(T, n_entries);
+  w.xs = c.take<uint16_t>(small ? 0 : static_cast<size_t>(n_entries) * int4_padded(H));
+  w.a = c.take<uint16_t>(static_cast<size_t>(n_entries) * int4_padded(I));
+  w.y = c.take<float>(small ? 0 : static_cast<size_t>(n_entries) * H);
   w.err = c.take<int32_t>(1);
   return w;
 }
@@ -911,6 +914,7 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   p.off = w.off;
   p.s_scatter = w.s_scatter;
   p.x_gather = w.x_gather;
+  p.xs = w.xs;
   p.a = w.a;
   p.y = w.y;
   p.out = out;
@@ -930,7 +934,7 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
     e = launch_route_scatter(expert_indices, token_indices, n_entries, K > 0 ? K : 1, per_tile, E, n_tiles,
                              w.route.tile_counts, w.off, w.s_scatter, w.s_rev, w.x_gather, st);
   if (e == cudaSuccess && token_indices) e = launch_token_offset(token_indices, T, n_entries, w.tok_off, st);
-  if (e == cudaSuccess) e = launch_int4_experts(p, st);
+  if (e == cudaSuccess) e = launch_int4_wide(p, st);
   return cuda_status(e, "moe_int4_forward");
 }
 

@@ -2,26 +2,11 @@
 // s * W2_e (silu(W1_e^gate x_t) * (W1_e^up x_t)), x and out bf16, the weights 4-bit codes with a scale
 // per group of input columns.
 //
-// Format.  w[n, k] = q[n, k] * s[n, k / group], q in [-7, 7], group 32, 64 or 128.  The scale is the
-// smallest number of 5 significant bits (at least 2^-126) that is >= amax / 7 of its group, so
-// q (3 bits) times s (5 bits) has at most 8 significant bits: every weight is exactly a bf16 number.
-// Taking 5 bits instead of bf16's 8 widens the step by 3% at most; in exchange the codes can be scaled
-// before or after the products, on any path, without a rounding of their own.
-//
-// Layout (int4_tile_bytes / int4_scales of them per expert).  Rows come in tiles of 16, columns in
-// blocks of 128 (both padded with zero weights).  A block of a tile is 2 x 512 bytes; in the half h,
-// lane l = 4 g + t of a warp owns 16 bytes = 4 words: row g and row g + 8 of the columns
-// 64 h + 8 t .. + 7, then of the columns 64 h + 32 + 8 t .. + 7.  Nibble i of a word holds the code + 8
-// of column 2 i, nibble i + 4 that of column 2 i + 1, so (word >> 4 i) & 0x000F000F is a pair of
-// neighbours in the halves of a register.  A column block's order inside the product does not matter
-// as long as x is read the same way: lane l reads 8 consecutive values of x (16 bytes) for each word
-// pair, and two m16n8k16 products consume them.  The scales of a block are [8][groups][2] bf16: for
-// g < 8 and each group of the block, rows g and g + 8 (one load of 4, 8 or 16 bytes a lane).  A GLU weight's prepared row 2 j is gate row j and 2 j + 1 up row j (the
-// interleaved order; a concatenated w1 is re-ordered when it is prepared).
+// The format and the layout are described in int4.cuh.  This file: preparing and expanding the weights,
+// and the layer for few tokens (int4_wide.cu has it for many).
 #include <type_traits>
 
-#include "common.cuh"
-#include "sonic_internal.h"
+#include "int4.cuh"
 
 namespace smb {
 
@@ -89,6 +74,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
       const int q = s > 0.0f ? static_cast<int>(rintf(__fdiv_rn(v[j], s))) : 0;
       word |= static_cast<uint32_t>(q + 8) << (4 * (j >> 1) + 16 * (j & 1));
     }
+    word = __funnelshift_l(word, word, 3);
     const int h = c >> 3, blk = (c >> 2) & 1, t = c & 3;
     s_word[warp][h * 128 + (4 * (r & 7) + t) * 4 + 2 * blk + (r >> 3)] = word;
     if (c % lanes_per_group == 0)
@@ -122,7 +108,8 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
     const int p = tile * 16 + r;
     if (p >= N || k0 >= K) continue;
     const int h = c >> 3, blk = (c >> 2) & 1, t = c & 3;
-    const uint32_t word = words[h * 128 + (4 * (r & 7) + t) * 4 + 2 * blk + (r >> 3)];
+    const uint32_t stored = words[h * 128 + (4 * (r & 7) + t) * 4 + 2 * blk + (r >> 3)];
+    const uint32_t word = __funnelshift_r(stored, stored, 3);
     const float s = __bfloat162float(
         ws[(et * k_blocks + kb) * gpb * 16 + ((r & 7) * gpb + c / lanes_per_group) * 2 + (r >> 3)]);
     uint32_t o[4];
@@ -137,30 +124,6 @@ __global__ void __launch_bounds__(32 * kPrepWarps)
 
 // ---------------------------------------------------------------------------------------------
 // products
-
-// The constants come from registers the compiler cannot look into: with two immediates it would spend two
-// instructions instead of one on the and-or.
-struct Int4Magic {
-  uint32_t mask, base;
-  __device__ __forceinline__ Int4Magic() {
-    asm volatile("mov.u32 %0, 0x000F000F;" : "=r"(mask));
-    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(base));
-  }
-};
-__device__ __forceinline__ uint32_t int4_pair_raw(const Int4Magic& c, uint32_t w, int i) {  // 128 + n
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "r"(c.mask), "r"(c.base));  // (a & b) | c
-  return r;
-}
-
-// Codes of word `w`, pair i (columns 2 i, 2 i + 1), as two bf16: 0x4300 is 128, whose last mantissa bit
-// is worth 1, so 0x4300 | n is 128 + n, and subtracting 136 leaves q = n - 8 exactly.
-__device__ __forceinline__ uint32_t int4_pair(const Int4Magic& c, uint32_t w, int i) {
-  const uint32_t u = int4_pair_raw(c, w, i);
-  const uint32_t off = 0x43084308u;
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&off));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
@@ -181,159 +144,6 @@ __device__ __forceinline__ void mma_bf16_16816_c(float (&d)[4], uint32_t a0, uin
 
 constexpr int kMvWarps = 8;
 constexpr int kMvThreads = 32 * kMvWarps;
-
-// acc[j][.] += rows of one tile times the tokens of n-tile j, over the column blocks [b0, b1).
-// wq: the tile's first block; sc: its scales; xrow[j]: this lane's token of n-tile j (null: none).
-template <int NT>
-__device__ __forceinline__ void mv_tile(const uint8_t* __restrict__ wq, const __nv_bfloat16* __restrict__ sc, int group,
-                                        int K, int b0, int b1, const __nv_bfloat16* const (&xrow)[NT],
-                                        float (&acc)[NT][4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Int4Magic magic;
-  for (int b = b0; b < b1; ++b) {
-    uint4 q[2];
-    q[0] = __ldg(reinterpret_cast<const uint4*>(wq + static_cast<size_t>(b) * 1024) + lane);
-    q[1] = __ldg(reinterpret_cast<const uint4*>(wq + static_cast<size_t>(b) * 1024) + 32 + lane);
-    const int gpb = 128 / group;
-    float part[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[j][i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {  // 32 columns each
-      const uint4 qh = q[s >> 1];
-      const uint32_t lo = s & 1 ? qh.z : qh.x, hi = s & 1 ? qh.w : qh.y;
-      const int k = b * 128 + 32 * s + 8 * t;
-      uint32_t a[4], c[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = int4_pair(magic, lo, i);
-        c[i] = int4_pair(magic, hi, i);
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        uint4 xv = make_uint4(0, 0, 0, 0);
-        if (xrow[j] && k < K) xv = __ldg(reinterpret_cast<const uint4*>(xrow[j] + k));
-        mma_bf16_16816(part[j], a[0], c[0], a[1], c[1], xv.x, xv.y);
-        mma_bf16_16816(part[j], a[2], c[2], a[3], c[3], xv.z, xv.w);
-      }
-      if (((s + 1) * 32) % group == 0) {  // end of a group: its sums times the rows' scales
-        const uint32_t s2 = __ldg(reinterpret_cast<const uint32_t*>(sc + static_cast<size_t>(b) * gpb * 16) +
-                                  g * gpb + (s * 32) / group);
-        const float slo = __uint_as_float(s2 << 16), shi = __uint_as_float(s2 & 0xFFFF0000u);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[j][0] = fmaf(slo, part[j][0], acc[j][0]);
-          acc[j][1] = fmaf(slo, part[j][1], acc[j][1]);
-          acc[j][2] = fmaf(shi, part[j][2], acc[j][2]);
-          acc[j][3] = fmaf(shi, part[j][3], acc[j][3]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part[j][i] = 0.0f;
-        }
-      }
-    }
-  }
-}
-
-struct MvArgs {
-  const uint8_t* wq;
-  const __nv_bfloat16* ws;
-  int group, N, K, n_tiles, k_blocks;  // prepared rows N, input columns K
-  const int32_t* freq;
-  const int32_t* off;
-  const int32_t* s_scatter;   // flat entry of a sorted position
-  const int32_t* x_gather;    // token of a sorted position
-  const __nv_bfloat16* x;     // up: tokens [T, K]; down: the intermediate [entries, K] in sorted order
-  int T;
-  const float* scores;        // down: by flat entry
-  __nv_bfloat16* a;           // up output [entries, N / 2], sorted order
-  float* y;                   // down output [entries, N] fp32, by flat entry, times the score
-  int* err;
-};
-
-// Tokens [c0, c0 + 8 NT) of expert e with one 16-row tile: the 8 warps split the columns, the sums meet
-// in shared memory.
-template <bool kUp, int NT>
-__device__ __forceinline__ void mv_chunk(const MvArgs& p, int e, int tile, int c0, int n, float* s_red) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int base = p.off[e] + c0;
-  const __nv_bfloat16* xrow[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int i = 8 * j + g;
-    xrow[j] = nullptr;
-    if (i < n) {
-      if (kUp) {
-        const int tok = p.x_gather[base + i];
-        if (tok >= 0 && tok < p.T)
-          xrow[j] = p.x + static_cast<size_t>(tok) * p.K;
-        else
-          atomicCAS(p.err, 0, kErrBadToken);
-      } else {
-        xrow[j] = p.x + static_cast<size_t>(base + i) * p.K;
-      }
-    }
-  }
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-  const size_t et = static_cast<size_t>(e) * p.n_tiles + tile;
-  mv_tile<NT>(p.wq + et * p.k_blocks * 1024, p.ws + et * p.k_blocks * (128 / p.group) * 16, p.group, p.K,
-              warp * p.k_blocks / kMvWarps, (warp + 1) * p.k_blocks / kMvWarps, xrow, acc);
-  constexpr int kLd = 8 * NT + 1;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    float* d = s_red + warp * 16 * kLd + 8 * j + 2 * t;
-    d[g * kLd] = acc[j][0];
-    d[g * kLd + 1] = acc[j][1];
-    d[(g + 8) * kLd] = acc[j][2];
-    d[(g + 8) * kLd + 1] = acc[j][3];
-  }
-  __syncthreads();
-  auto total = [&](int row, int i) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kMvWarps; ++w) v += s_red[w * 16 * kLd + row * kLd + i];
-    return v;
-  };
-  if (kUp) {
-    for (int o = threadIdx.x; o < 8 * n; o += kMvThreads) {
-      const int i = o >> 3, r = o & 7;
-      const int col = tile * 8 + r;
-      if (col >= p.N / 2) continue;
-      const float gate = total(2 * r, i), up = total(2 * r + 1, i);
-      p.a[static_cast<size_t>(base + i) * (p.N / 2) + col] = __float2bfloat16_rn(gate / (1.0f + __expf(-gate)) * up);
-    }
-  } else {
-    for (int o = threadIdx.x; o < 16 * n; o += kMvThreads) {
-      const int i = o >> 4, r = o & 15;
-      const int col = tile * 16 + r;
-      if (col >= p.N) continue;
-      const int f = p.s_scatter[base + i];
-      p.y[static_cast<size_t>(f) * p.N + col] = p.scores[f] * total(r, i);
-    }
-  }
-}
-
-template <bool kUp>
-__global__ void __launch_bounds__(kMvThreads) mv_kernel(const MvArgs p) {
-  __shared__ float s_red[kMvWarps * 16 * 33];
-  const int e = blockIdx.y, tile = blockIdx.x;
-  const int n_e = p.freq[e];
-  for (int c0 = 0; c0 < n_e; c0 += 32) {
-    const int n = min(32, n_e - c0);
-    if (n <= 8)
-      mv_chunk<kUp, 1>(p, e, tile, c0, n, s_red);
-    else if (n <= 16)
-      mv_chunk<kUp, 2>(p, e, tile, c0, n, s_red);
-    else
-      mv_chunk<kUp, 4>(p, e, tile, c0, n, s_red);
-  }
-}
 
 // ---------------------------------------------------------------------------------------------
 // Few tokens.  Two launches: the up projection and the down projection with the sum over a token's
@@ -515,28 +325,6 @@ constexpr int kDepth = MT == 1 ? 6 : 4;
 template <int MT, int GPB>
 constexpr int kStage = MT * (1024 + 128 * GPB);
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-template <int kBytes>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
 // src: the lane's piece of the block in the first tile's codes, sc: its scales; the second tile's lie
 // tile2 blocks further on.
 template <int MT, int GPB>
@@ -564,20 +352,15 @@ __device__ __forceinline__ uint4 load_x(const __nv_bfloat16* xrow, int b, int s,
   return kUp ? __ldg(reinterpret_cast<const uint4*>(xrow + k)) : ld_plain(xrow + k);
 }
 
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-
 // One stage's products.  With few tokens (NT <= 2) the instructions per weight count: a group's sums are
-// scaled, in fp32, and the offset of the codes (128 + n stands for n - 8) is taken from the sums too, which
-// start at -136 times the sum of x, itself a product with a constant.  With more tokens the codes lose
+// scaled, in fp32, and the offset of the codes (16 + n stands for q + 24) is taken from the sums too, which
+// start at -24 times the sum of x, itself a product with a constant.  With more tokens the codes lose
 // their offset and are scaled (both exact), which leaves the sums of all groups in one accumulator.
 template <int MT, int NT, int GPB, bool kUp>
 __device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage, int b, int K, bool whole, const __nv_bfloat16* const* xrow,
                                           const uint4* xv, float (*acc)[MT][4]) {
   constexpr bool kSums = NT <= 2;
-  constexpr uint32_t kMinus136 = 0xC308C308u;
+  constexpr uint32_t kMinus24 = 0xC1C0C1C0u;
   const int lane = threadIdx.x & 31;
   float part[kSums ? NT : 1][MT][4];
   uint4 q[MT];
@@ -603,16 +386,21 @@ __device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (s % 2 == 0) q[m] = lds128(stage + 1024 * m + 256 * s + 16 * lane);
+      const uint32_t wl = s & 1 ? q[m].z : q[m].x, wh = s & 1 ? q[m].w : q[m].y;
+      if constexpr (kSums) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t wl = s & 1 ? q[m].z : q[m].x, wh = s & 1 ? q[m].w : q[m].y;
-        if constexpr (kSums) {
-          lo[m][i] = int4_pair_raw(magic, wl, i);
-          hi[m][i] = int4_pair_raw(magic, wh, i);
-        } else {
-          const uint32_t sw = s2[m][s / (4 / GPB)];
-          lo[m][i] = mul_bf16x2(int4_pair(magic, wl, i), __byte_perm(sw, 0, 0x1010));
-          hi[m][i] = mul_bf16x2(int4_pair(magic, wh, i), __byte_perm(sw, 0, 0x3232));
+        for (int i = 0; i < 4; ++i) {
+          lo[m][i] = int4_raw(magic, wl, i);
+          hi[m][i] = int4_raw(magic, wh, i);
+        }
+      } else {
+        const uint32_t sw = s2[m][s / (4 / GPB)];
+        const __nv_bfloat162 sl = int4_scale2(sw, 0), sh = int4_scale2(sw, 1);
+        const __nv_bfloat162 ml = int4_m24(sl), mh = int4_m24(sh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[m][i] = int4_scaled(magic, wl, i, sl, ml);
+          hi[m][i] = int4_scaled(magic, wh, i, sh, mh);
         }
       }
     }
@@ -627,8 +415,8 @@ __device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage
         }
       } else {
         float c[4];
-        mma_bf16_16816_c(c, kMinus136, kMinus136, kMinus136, kMinus136, x.x, x.y, 0.0f, 0.0f, 0.0f, 0.0f);
-        mma_bf16_16816(c, kMinus136, kMinus136, kMinus136, kMinus136, x.z, x.w);
+        mma_bf16_16816_c(c, kMinus24, kMinus24, kMinus24, kMinus24, x.x, x.y, 0.0f, 0.0f, 0.0f, 0.0f);
+        mma_bf16_16816(c, kMinus24, kMinus24, kMinus24, kMinus24, x.z, x.w);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           float(&d)[4] = part[j][m];
@@ -762,8 +550,6 @@ __device__ __forceinline__ void stream_items(const SmallArgs& p, const SmallPlan
     }
   }
 }
-
-__device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
 
 // Up projection and SwiGLU: a persistent grid, item = (slot, MT row tiles).  With ksplit > 1 (few items)
 // adjacent warps of a CTA share a tile's columns and their sums meet in shared memory.
@@ -917,29 +703,6 @@ __global__ void __launch_bounds__(kMvThreads, 2) small_down_kernel(const SmallAr
   }
 }
 
-// out[t] = sum of the rows y[f] of t's entries, f in [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]),
-// in entry order, rounded once.  Entries whose expert or token was rejected have no row.
-__global__ void __launch_bounds__(256)
-    int4_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
-                        const int32_t* __restrict__ experts, int E, __nv_bfloat16* __restrict__ out) {
-  const int t = blockIdx.y;
-  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-  if (c >= H) return;
-  const int f0 = tok_off ? tok_off[t] : t * K, f1 = tok_off ? tok_off[t + 1] : (t + 1) * K;
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int f = f0; f < f1; ++f) {
-    const int e = experts[f];
-    if (e < 0 || e >= E) continue;
-    const float4 v = *reinterpret_cast<const float4*>(y + static_cast<size_t>(f) * H + c);
-    s.x += v.x;
-    s.y += v.y;
-    s.z += v.z;
-    s.w += v.w;
-  }
-  *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + c) =
-      make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
-}
-
 }  // namespace
 
 int int4_row_tiles(int N) { return ceil_div(N, 16); }
@@ -1064,52 +827,6 @@ cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st) {
   if (p.T <= 8) return launch_small<2, 1>(u, p.group1, d, p.group2, st);
   if (p.T <= 16) return launch_small<2, 2>(u, p.group1, d, p.group2, st);
   return launch_small<2, 4>(u, p.group1, d, p.group2, st);
-}
-
-cudaError_t launch_int4_experts(const Int4Args& p, cudaStream_t st) {
-  MvArgs u{};
-  u.wq = p.w1q;
-  u.ws = static_cast<const __nv_bfloat16*>(p.w1s);
-  u.group = p.group1;
-  u.N = 2 * p.I;
-  u.K = p.H;
-  u.n_tiles = int4_row_tiles(u.N);
-  u.k_blocks = int4_col_blocks(u.K);
-  u.freq = p.freq;
-  u.off = p.off;
-  u.s_scatter = p.s_scatter;
-  u.x_gather = p.x_gather;
-  u.x = static_cast<const __nv_bfloat16*>(p.x);
-  u.T = p.T;
-  u.a = static_cast<__nv_bfloat16*>(p.a);
-  u.err = p.err;
-  MvArgs d = u;
-  d.wq = p.w2q;
-  d.ws = static_cast<const __nv_bfloat16*>(p.w2s);
-  d.group = p.group2;
-  d.N = p.H;
-  d.K = p.I;
-  d.n_tiles = int4_row_tiles(d.N);
-  d.k_blocks = int4_col_blocks(d.K);
-  d.x = u.a;
-  d.scores = p.scores;
-  d.y = p.y;
-  mv_kernel<true><<<dim3(u.n_tiles, p.E), kMvThreads, 0, st>>>(u);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  mv_kernel<false><<<dim3(d.n_tiles, p.E), kMvThreads, 0, st>>>(d);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  for (int t0 = 0; t0 < p.T; t0 += 32768) {  // grid.y limit
-    const int n = p.T - t0 < 32768 ? p.T - t0 : 32768;
-    int4_combine_kernel<<<dim3(ceil_div(p.H, 1024), n), 256, 0, st>>>(
-        p.y + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K * p.H), n, p.H, p.K,
-        p.tok_off ? p.tok_off + t0 : nullptr, p.experts + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K), p.E,
-        static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t0) * p.H);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
 }
 
 }  // namespace smb

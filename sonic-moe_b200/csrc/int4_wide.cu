@@ -1,0 +1,496 @@
+// Expert products with 4-bit weights for many tokens (format and layout: int4.cuh; few tokens: int4.cu).
+//
+// Grouped GEMMs on tcgen05 whose first operand is the weight: D[128 rows, tokens] = W[128, K] x[tokens, K]^T.
+// The codes go from global memory through shared memory into registers, become bf16 there (exact, scale
+// included) and are stored to tensor memory, from where the MMA reads its A operand; x comes through TMA
+// into 128-byte-swizzled shared memory.  Keeping A out of shared memory is what makes this bound by the
+// weights' bytes rather than by shared memory: at 64 tokens a 128 x 64 step moves 4 KB of codes, and
+// writing its 16 KB of bf16 to shared memory and reading it back would take twice as long as HBM does.
+//
+// The columns inside a block of 32 are permuted on the way (both operands alike, the product does not
+// see it): a lane of a dequantising warp holds 8 consecutive columns as 4 pairs, and the 16-lane x
+// 128-bit store to tensor memory takes one pair of each of 4 lanes, so column 8 t + 2 i + e sits at
+// place 8 i + 2 t + e.  x is gathered into expert order and permuted by wide_gather_kernel; the up
+// projection writes its intermediate in that order.
+//
+// Roles per CTA (448 threads, one CTA per SM):
+//   warps 0-7   dequantise: warp w stores rows 32 (w % 4) .. + 31, half w / 4 of each 128-column block
+//   warps 8-11  epilogue: rows 32 (w % 4) .. of the accumulator (two accumulators of 128 columns)
+//   warp 12     TMA producer of x,  warp 13  MMA issuer (and tensor memory allocation)
+// Work items (expert, 128 rows, up to 128 of its tokens), rows fastest, static round robin; the items of
+// an expert's token chunks follow each other, so their second reading of the weights is from L2.
+// Every wait is bounded; after a time-out the kernel records an error, drains and returns.
+#include "int4.cuh"
+
+namespace smb {
+
+namespace {
+
+constexpr int kWdThreads = 448;
+constexpr int kWdStages = 6;  // 64-column steps of x (shared memory) and of the weights (tensor memory)
+constexpr int kWdN = 128;     // tokens of an item at most
+constexpr int kWdBStage = kWdN * 128;
+constexpr int kWdRing = 8;    // half blocks of codes in flight per dequantising warp
+constexpr uint32_t kWdTmemA = 256;  // accumulators 0-127 and 128-255, A stages of 32 columns from here
+
+template <int GPB>
+struct WdRing {
+  static constexpr int kSc = GPB == 4 ? 2 : 1;  // scale words of a lane for half a block of one row tile
+  static constexpr int kStage = 2 * (512 + 128 * kSc);
+  static constexpr int kBytes = 8 * kWdRing * kStage;
+};
+
+struct WdArgs {
+  const uint8_t* wq;
+  const __nv_bfloat16* ws;
+  int N, n_tiles, k_blocks;  // prepared rows, their 16-row tiles, column blocks
+  int E, m_tiles;
+  const int32_t* freq;
+  const int32_t* off;
+  const int32_t* s_scatter;
+  const float* scores;
+  __nv_bfloat16* a;  // up output [entries, a_ld], sorted order, permuted columns, zero beyond N / 2
+  int a_ld;
+  float* y;  // down output [entries, N] by flat entry, times the score
+  int* err;
+};
+
+struct WdItem {
+  int e, mt, base, n;
+};
+
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::f16 instruction descriptor: bf16 x bf16 -> f32, both operands K-major.
+__device__ __forceinline__ uint32_t wd_idesc(int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+// 16 lanes x 32 columns: lane 4 g + t of the warp gives columns 4 c + t of rows g (r[2 c]) and g + 8 (r[2 c + 1]).
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Place of column k (< 32) of a block of 32 in the permuted order.
+__device__ __forceinline__ int wd_place(int k) { return 8 * ((k >> 1) & 3) + 2 * (k >> 3) + (k & 1); }
+
+template <bool kUp, int GPB>
+__global__ void __launch_bounds__(kWdThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const WdArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_a[kWdStages], full_b[kWdStages], empty[kWdStages], tfull[2], tempty[2], drain;
+  __shared__ uint32_t tmem_holder;
+  __shared__ int32_t s_warp[kWdThreads / 32];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* rings = smem + kWdStages * kWdBStage;
+  int32_t* pre = reinterpret_cast<int32_t*>(rings + WdRing<GPB>::kBytes);  // [E + 1] chunks before each expert
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < kWdStages; ++s) {
+      mbar_init(&full_a[s], 4);
+      mbar_init(&full_b[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmap_x);
+  }
+  if (warp == 13) {
+    tmem_alloc(&tmem_holder, 512);
+    tmem_relinquish();
+  }
+  {  // chunks of kWdN tokens per expert, exclusive prefix
+    const int per = (p.E + kWdThreads - 1) / kWdThreads;
+    const int e0 = min(p.E, tid * per), e1 = min(p.E, e0 + per);
+    int c = 0;
+    for (int e = e0; e < e1; ++e) c += (p.freq[e] + kWdN - 1) / kWdN;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    int run = inc - c;
+    for (int w = 0; w < warp; ++w) run += s_warp[w];
+    for (int e = e0; e < e1; ++e) {
+      pre[e] = run;
+      run += (p.freq[e] + kWdN - 1) / kWdN;
+    }
+    if (tid == kWdThreads - 1) pre[p.E] = run;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  const int items = pre[p.E] * p.m_tiles;
+  auto item_of = [&](int i) {
+    WdItem it;
+    const int c = i / p.m_tiles;
+    it.mt = i - c * p.m_tiles;
+    int lo = 0, hi = p.E;  // pre[lo] <= c < pre[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= c)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    it.e = lo;
+    const int done = (c - pre[lo]) * kWdN;
+    it.base = p.off[lo] + done;
+    it.n = min(kWdN, p.freq[lo] - done);
+    return it;
+  };
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- dequantise
+    constexpr int kSc = WdRing<GPB>::kSc, kStage = WdRing<GPB>::kStage;
+    const Int4Magic magic;
+    const int quarter = warp & 3, half = warp >> 2, g = lane >> 2;
+    const uint32_t ring = smem_u32(rings) + warp * kWdRing * kStage;
+    int l_item = blockIdx.x, l_b = 0, l_stage = 0, u_stage = 0;
+    const uint8_t* l_src[2] = {};
+    const __nv_bfloat16* l_sc[2] = {};
+    bool l_on[2] = {};
+    auto open = [&] {
+      if (l_item >= items) return;
+      const WdItem it = item_of(l_item);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int tile = it.mt * 8 + 2 * quarter + j;
+        l_on[j] = tile < p.n_tiles;
+        const size_t blk = (static_cast<size_t>(it.e) * p.n_tiles + (l_on[j] ? tile : 0)) * p.k_blocks;
+        l_src[j] = p.wq + blk * 1024 + half * 512 + 16 * lane;
+        l_sc[j] = p.ws + blk * (GPB * 16) + g * (GPB * 2) + (GPB == 4 ? 4 * half : GPB == 2 ? 2 * half : 0);
+      }
+    };
+    auto fill = [&] {
+      if (l_item < items) {
+        const uint32_t st = ring + l_stage * kStage;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t sd = st + 1024 + j * 128 * kSc + 4 * kSc * lane;
+          if (l_on[j]) {
+            cp_async16(st + 512 * j + 16 * lane, l_src[j]);
+            cp_async_small<4 * kSc>(sd, l_sc[j]);
+          } else {  // rows past the last tile: any codes, scale 0
+#pragma unroll
+            for (int i = 0; i < kSc; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sd + 4 * i), "r"(0) : "memory");
+          }
+          l_src[j] += 1024;
+          l_sc[j] += GPB * 16;
+        }
+        if (++l_stage == kWdRing) l_stage = 0;
+        if (++l_b == p.k_blocks) {
+          l_b = 0;
+          l_item += gridDim.x;
+          open();
+        }
+      }
+      cp_async_commit();
+    };
+    open();
+#pragma unroll
+    for (int d = 0; d < kWdRing - 1; ++d) fill();
+    // Steps of an item: 2 k_blocks, an even number like the ring's, so that each half always meets the
+    // same stages and waits for every use of them (a parity wait may not skip one).
+    int step = half;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+      for (int b = 0; b < p.k_blocks; ++b, step += 2) {
+        fill();  // the stage freed by the step before
+        cp_async_wait<kWdRing - 1>();
+        const uint32_t st = ring + u_stage * kStage;
+        if (++u_stage == kWdRing) u_stage = 0;
+        uint32_t r[2][16];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 q = lds128(st + 512 * j + 16 * lane);
+          const uint32_t sd = st + 1024 + j * 128 * kSc + 4 * kSc * lane;
+          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {  // 32 columns
+            const uint32_t sw = lds32(sd + (kSc == 2 ? 4 * k : 0));
+            const __nv_bfloat162 sl = int4_scale2(sw, 0), sh = int4_scale2(sw, 1);
+            const __nv_bfloat162 ml = int4_m24(sl), mh = int4_m24(sh);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              r[j][2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
+              r[j][2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
+            }
+          }
+        }
+        const int s = step % kWdStages;
+        if (!mbar_wait(&empty[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t dst = tmem + kWdTmemA + 32 * s + (static_cast<uint32_t>(32 * quarter) << 16);
+        tmem_st_16x32(dst, r[0]);
+        tmem_st_16x32(dst + (16u << 16), r[1]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_a[s]);
+      }
+    }
+    cp_async_wait<0>();
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- epilogue
+    const int quarter = warp & 3;
+    int li = 0;
+    for (int i = blockIdx.x; i < items; i += gridDim.x, ++li) {
+      const WdItem it = item_of(i);
+      const int buf = li & 1;
+      if (!mbar_wait(&tfull[buf], (li >> 1) & 1, p.err, kErrTimeoutEpilogue)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * kWdN + (static_cast<uint32_t>(32 * quarter) << 16);
+      for (int c0 = 0; c0 < it.n; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(acc + c0, v);
+        tmem_ld_wait();
+        const int n = min(32, it.n - c0);
+        if (kUp) {
+          // even lanes hold gates, odd lanes the ups of the same output column: a pair finishes two tokens
+          const bool odd = lane & 1;
+          const int col = it.mt * 64 + quarter * 16 + (lane >> 1);
+          __nv_bfloat16* dst = p.a + static_cast<size_t>(it.base + c0) * p.a_ld + (col & ~31) + wd_place(col & 31);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float v0 = __uint_as_float(v[c]), v1 = __uint_as_float(v[c + 1]);
+            const float o = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+            const float r = odd ? silu_mul(o, v1) : silu_mul(v0, o);
+            const int t = c + (odd ? 1 : 0);
+            if (t < n) dst[static_cast<size_t>(t) * p.a_ld] = __float2bfloat16_rn(r);
+          }
+        } else {
+          const int row = it.mt * 128 + quarter * 32 + lane;
+          int f = 0;
+          float sc = 0.0f;
+          if (lane < n) {
+            f = p.s_scatter[it.base + c0 + lane];
+            sc = p.scores[f];
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (c >= n) break;
+            const int fc = __shfl_sync(0xffffffffu, f, c);
+            const float s = __shfl_sync(0xffffffffu, sc, c);
+            if (row < p.N) p.y[static_cast<size_t>(fc) * p.N + row] = s * __uint_as_float(v[c]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+    }
+  } else if (warp == 12) {
+    // ---------------------------------------------------------------- TMA producer of x
+    if (lane == 0) {
+      const uint64_t policy = policy_evict_last();  // every row tile of the expert reads it
+      int step = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
+        const WdItem it = item_of(i);
+        const int boxes = (it.n + 15) / 16;
+        for (int k = 0; k < 2 * p.k_blocks; ++k, ++step) {
+          const int s = step % kWdStages;
+          if (!mbar_wait(&empty[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full_b[s], boxes * 2048);
+          for (int r = 0; r < boxes; ++r)
+            tma_load_2d(smem + s * kWdBStage + r * 2048, &tmap_x, &full_b[s], k * 64, it.base + 16 * r, policy);
+        }
+      }
+      if (!ok)  // let the loads already issued land before shared memory goes away
+        for (int j = max(0, step - kWdStages); j < step; ++j)
+          mbar_wait_ns(&full_b[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
+    }
+  } else if (lane == 0) {
+    // ---------------------------------------------------------------- MMA issuer
+    int step = 0, li = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
+      const WdItem it = item_of(i);
+      const uint32_t idesc = wd_idesc((it.n + 15) & ~15);
+      const int buf = li & 1;
+      if (!mbar_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      for (int k = 0; k < 2 * p.k_blocks; ++k, ++step) {
+        const int s = step % kWdStages;
+        const uint32_t ph = (step / kWdStages) & 1;
+        if (!mbar_wait(&full_b[s], ph, p.err, kErrTimeoutMma) || !mbar_wait(&full_a[s], ph, p.err, kErrTimeoutMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t bd = sdesc_sw128(smem_u32(smem + s * kWdBStage));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
+          tc_mma_bf16_ts(tmem + buf * kWdN, tmem + kWdTmemA + 32 * s + 8 * kk, bd + 2 * kk, idesc,
+                         (k | kk) != 0 ? 1u : 0u);
+        tc_commit(&empty[s]);
+      }
+      if (ok) tc_commit(&tfull[buf]);
+    }
+    tc_commit(&drain);  // every MMA has finished before tensor memory is freed
+    mbar_wait_ns(&drain, 0, 100000000ull);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// x rows in expert order with permuted columns: xs[pos][32 b + wd_place(k)] = x[token(pos)][32 b + k], zero
+// beyond K.  One thread per (position, block of 32 columns): a 4 x 4 transpose of column pairs.
+__global__ void __launch_bounds__(256)
+    wide_gather_kernel(const __nv_bfloat16* __restrict__ x, int T, int K, const int32_t* __restrict__ x_gather,
+                       const int32_t* __restrict__ freq, const int32_t* __restrict__ off, int E, int blocks,
+                       __nv_bfloat16* __restrict__ xs, int* err) {
+  const int total = off[E - 1] + freq[E - 1];  // entries that were not rejected
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const int pos = static_cast<int>(i / blocks), b = static_cast<int>(i % blocks);
+  if (pos >= total) return;
+  const int tok = x_gather[pos];
+  const bool ok = tok >= 0 && tok < T;
+  if (!ok && b == 0) atomicCAS(err, 0, kErrBadToken);
+  uint32_t w[4][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    const int k = 32 * b + 8 * t;
+    if (ok && k < K) v = *reinterpret_cast<const uint4*>(x + static_cast<size_t>(tok) * K + k);
+    w[t][0] = v.x;
+    w[t][1] = v.y;
+    w[t][2] = v.z;
+    w[t][3] = v.w;
+  }
+  uint4* dst = reinterpret_cast<uint4*>(xs + (static_cast<size_t>(pos) * blocks + b) * 32);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) dst[c] = make_uint4(w[0][c], w[1][c], w[2][c], w[3][c]);
+}
+
+// out[t] = sum of the rows y[f] of t's entries, f in [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]),
+// in entry order, rounded once.  Entries whose expert or token was rejected have no row.
+__global__ void __launch_bounds__(256)
+    int4_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
+                        const int32_t* __restrict__ experts, int E, __nv_bfloat16* __restrict__ out) {
+  const int t = blockIdx.y;
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+  if (c >= H) return;
+  const int f0 = tok_off ? tok_off[t] : t * K, f1 = tok_off ? tok_off[t + 1] : (t + 1) * K;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int f = f0; f < f1; ++f) {
+    const int e = experts[f];
+    if (e < 0 || e >= E) continue;
+    const float4 v = *reinterpret_cast<const float4*>(y + static_cast<size_t>(f) * H + c);
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + c) =
+      make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
+}
+
+template <bool kUp, int GPB>
+cudaError_t launch_wide(const CUtensorMap& tx, const WdArgs& p, int grid, cudaStream_t st) {
+  const int smem = 1024 + kWdStages * kWdBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
+  auto kern = wide_kernel<kUp, GPB>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kWdThreads, smem, st>>>(tx, p);
+  return cudaGetLastError();
+}
+
+template <bool kUp>
+cudaError_t launch_wide(WdArgs p, const void* x, int ld, int n_entries, int group, cudaStream_t st) {
+  CUtensorMap tx;
+  if (!encode_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, static_cast<uint64_t>(ld),
+                      static_cast<uint64_t>(n_entries), 64, 16, true))
+    return cudaErrorInvalidValue;
+  const long long most = (n_entries / kWdN + static_cast<long long>(p.E < n_entries ? p.E : n_entries)) * p.m_tiles;
+  const int sms = gemm_grid_sms();
+  const int grid = most < sms ? static_cast<int>(most) : sms;
+  return group == 32   ? launch_wide<kUp, 4>(tx, p, grid, st)
+         : group == 64 ? launch_wide<kUp, 2>(tx, p, grid, st)
+                       : launch_wide<kUp, 1>(tx, p, grid, st);
+}
+
+}  // namespace
+
+int int4_padded(int K) { return int4_col_blocks(K) * 128; }
+
+cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
+  const int blocks = int4_padded(p.H) / 32;
+  const long long threads = static_cast<long long>(p.n_entries) * blocks;
+  wide_gather_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, st>>>(
+      static_cast<const __nv_bfloat16*>(p.x), p.T, p.H, p.x_gather, p.freq, p.off, p.E, blocks,
+      static_cast<__nv_bfloat16*>(p.xs), p.err);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  WdArgs u{};
+  u.wq = p.w1q;
+  u.ws = static_cast<const __nv_bfloat16*>(p.w1s);
+  u.N = 2 * p.I;
+  u.n_tiles = int4_row_tiles(u.N);
+  u.k_blocks = int4_col_blocks(p.H);
+  u.E = p.E;
+  u.m_tiles = int4_padded(p.I) / 64;  // the padding of the intermediate is written too (zeros)
+  u.freq = p.freq;
+  u.off = p.off;
+  u.s_scatter = p.s_scatter;
+  u.scores = p.scores;
+  u.a = static_cast<__nv_bfloat16*>(p.a);
+  u.a_ld = int4_padded(p.I);
+  u.y = p.y;
+  u.err = p.err;
+  WdArgs d = u;
+  d.wq = p.w2q;
+  d.ws = static_cast<const __nv_bfloat16*>(p.w2s);
+  d.N = p.H;
+  d.n_tiles = int4_row_tiles(d.N);
+  d.k_blocks = int4_col_blocks(p.I);
+  d.m_tiles = ceil_div(d.N, 128);
+  e = launch_wide<true>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st);
+  if (e != cudaSuccess) return e;
+  e = launch_wide<false>(d, p.a, u.a_ld, p.n_entries, p.group2, st);
+  if (e != cudaSuccess) return e;
+  for (int t0 = 0; t0 < p.T; t0 += 32768) {  // grid.y limit
+    const int n = p.T - t0 < 32768 ? p.T - t0 : 32768;
+    int4_combine_kernel<<<dim3(ceil_div(p.H, 1024), n), 256, 0, st>>>(
+        p.y + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K * p.H), n, p.H, p.K,
+        p.tok_off ? p.tok_off + t0 : nullptr, p.experts + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K), p.E,
+        static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t0) * p.H);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace smb
