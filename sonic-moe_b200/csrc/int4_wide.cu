@@ -4,8 +4,8 @@
 // The codes go from global memory through shared memory into registers, become bf16 there (exact, scale
 // included) and are stored to tensor memory, from where the MMA reads its A operand; x comes through TMA
 // into 128-byte-swizzled shared memory.  Keeping A out of shared memory is what makes this bound by the
-// weights' bytes rather than by shared memory: at 64 tokens a 128 x 64 step moves 4 KB of codes, and
-// writing its 16 KB of bf16 to shared memory and reading it back would take twice as long as HBM does.
+// weights' bytes rather than by shared memory: at 64 tokens a 128 x 128 step moves 8 KB of codes, and
+// writing its 32 KB of bf16 to shared memory and reading it back would take twice as long as HBM does.
 //
 // The columns inside a block of 32 are permuted on the way (both operands alike, the product does not
 // see it): a lane of a dequantising warp holds 8 consecutive columns as 4 pairs, and the 16-lane x
@@ -13,11 +13,13 @@
 // place 8 i + 2 t + e.  x is gathered into expert order and permuted by wide_gather_kernel; the up
 // projection writes its intermediate in that order.
 //
-// Roles per CTA (448 threads, one CTA per SM):
-//   warps 0-7   dequantise: warp w stores rows 32 (w % 4) .. + 31, half w / 4 of each 128-column block
-//   warps 8-11  epilogue: rows 32 (w % 4) .. of the accumulator (two accumulators of 128 columns)
-//   warp 12     TMA producer of x,  warp 13  MMA issuer (and tensor memory allocation)
-// Work items (expert, 128 rows, up to 128 of its tokens), rows fastest, static round robin; the items of
+// Roles per CTA (704 threads, one CTA per SM):
+//   warps 0-15   dequantise: warp w stores rows 32 (w % 4) .. + 31 of every 4th step of 128 columns
+//   warps 16-19  epilogue: rows 32 (w % 4) .. of the accumulator (two accumulators of 64 columns)
+//   warp 20      TMA producer of x,  warp 21  MMA issuer (and tensor memory allocation)
+// A step is as long as it is (8 MMAs of 16 columns) because the issuer's waits and commit cost some
+// hundred cycles whatever they guard; steps of 64 columns were bound by them.
+// Work items (expert, 128 rows, up to 64 of its tokens), rows fastest, static round robin; the items of
 // an expert's token chunks follow each other, so their second reading of the weights is from L2.
 // Every wait is bounded; after a time-out the kernel records an error, drains and returns.
 #include "int4.cuh"
@@ -26,18 +28,21 @@ namespace smb {
 
 namespace {
 
-constexpr int kWdThreads = 448;
-constexpr int kWdStages = 6;  // 64-column steps of x (shared memory) and of the weights (tensor memory)
-constexpr int kWdN = 128;     // tokens of an item at most
-constexpr int kWdBStage = kWdN * 128;
-constexpr int kWdRing = 8;    // half blocks of codes in flight per dequantising warp
-constexpr uint32_t kWdTmemA = 256;  // accumulators 0-127 and 128-255, A stages of 32 columns from here
+constexpr int kWdDeqWarps = 16;
+constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps make a step's 128 rows
+constexpr int kWdThreads = 32 * (kWdDeqWarps + 6);
+constexpr int kWdStages = 4;  // 128-column steps of x (shared memory) and of the weights (tensor memory)
+constexpr int kWdN = 64;      // tokens of an item at most
+constexpr int kWdBHalf = kWdN * 128;  // 64 columns of x
+constexpr int kWdBStage = 2 * kWdBHalf;
+constexpr uint32_t kWdTmemA = 256;  // accumulators at 0 and 64, A stages of 64 columns from here
+static_assert(kWdStages == kWdGroups, "a group of dequantising warps owns a stage");
 
 template <int GPB>
 struct WdRing {
-  static constexpr int kSc = GPB == 4 ? 2 : 1;  // scale words of a lane for half a block of one row tile
-  static constexpr int kStage = 2 * (512 + 128 * kSc);
-  static constexpr int kBytes = 8 * kWdRing * kStage;
+  static constexpr int kStage = 2 * (1024 + 128 * GPB);  // a step of 2 row tiles, GPB scale words a lane
+  static constexpr int kDepth = GPB == 4 ? 3 : 4;        // steps of codes in flight per dequantising warp
+  static constexpr int kBytes = kWdDeqWarps * kDepth * kStage;
 };
 
 struct WdArgs {
@@ -83,14 +88,28 @@ __device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+// A wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, where));
+}
+
+// Tokens of one of an expert's ceil(n / kWdN) chunks: equal shares, whole 16s but for the last.
+__device__ __forceinline__ int wd_share(int n, int chunks) { return ((n + chunks - 1) / chunks + 15) & ~15; }
+
 // Place of column k (< 32) of a block of 32 in the permuted order.
 __device__ __forceinline__ int wd_place(int k) { return 8 * ((k >> 1) & 3) + 2 * (k >> 3) + (k & 1); }
 
 template <bool kUp, int GPB>
 __global__ void __launch_bounds__(kWdThreads, 1)
-    wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const WdArgs p) {
+    wide_kernel(const __grid_constant__ CUtensorMap tmap_x16, const __grid_constant__ CUtensorMap tmap_x64,
+                const WdArgs p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_a[kWdStages], full_b[kWdStages], empty[kWdStages], tfull[2], tempty[2], drain;
+  __shared__ uint64_t full[kWdStages], empty[kWdStages], tfull[2], tempty[2], drain;
   __shared__ uint32_t tmem_holder;
   __shared__ int32_t s_warp[kWdThreads / 32];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -101,8 +120,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < kWdStages; ++s) {
-      mbar_init(&full_a[s], 4);
-      mbar_init(&full_b[s], 1);
+      mbar_init(&full[s], 4 + 1);  // a group's warps and the producer of x
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -111,9 +129,10 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     }
     mbar_init(&drain, 1);
     fence_mbar_init();
-    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_x16);
+    prefetch_tmap(&tmap_x64);
   }
-  if (warp == 13) {
+  if (warp == kWdDeqWarps + 5) {
     tmem_alloc(&tmem_holder, 512);
     tmem_relinquish();
   }
@@ -156,32 +175,38 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         hi = mid;
     }
     it.e = lo;
-    const int done = (c - pre[lo]) * kWdN;
+    const int n = p.freq[lo], share = wd_share(n, pre[lo + 1] - pre[lo]);
+    const int done = (c - pre[lo]) * share;
     it.base = p.off[lo] + done;
-    it.n = min(kWdN, p.freq[lo] - done);
+    it.n = min(share, n - done);
     return it;
   };
 
-  if (warp < 8) {
+  if (warp < kWdDeqWarps) {
     // ---------------------------------------------------------------- dequantise
-    constexpr int kSc = WdRing<GPB>::kSc, kStage = WdRing<GPB>::kStage;
+    // Steps are numbered through all items of the CTA; group warp / 4 takes every 4th of them, and with
+    // them one stage.
+    constexpr int kStage = WdRing<GPB>::kStage, kDepth = WdRing<GPB>::kDepth;
     const Int4Magic magic;
-    const int quarter = warp & 3, half = warp >> 2, g = lane >> 2;
-    const uint32_t ring = smem_u32(rings) + warp * kWdRing * kStage;
-    int l_item = blockIdx.x, l_b = 0, l_stage = 0, u_stage = 0;
+    const int quarter = warp & 3, group = warp >> 2, g = lane >> 2;
+    const uint32_t ring = smem_u32(rings) + warp * kDepth * kStage;
+    int l_item = blockIdx.x, l_b = group, l_stage = 0, u_stage = 0;
     const uint8_t* l_src[2] = {};
     const __nv_bfloat16* l_sc[2] = {};
     bool l_on[2] = {};
-    auto open = [&] {
+    auto open = [&] {  // the item of block l_b
+      const int skip = l_b / p.k_blocks;
+      l_item += skip * gridDim.x;
+      l_b -= skip * p.k_blocks;
       if (l_item >= items) return;
       const WdItem it = item_of(l_item);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int tile = it.mt * 8 + 2 * quarter + j;
         l_on[j] = tile < p.n_tiles;
-        const size_t blk = (static_cast<size_t>(it.e) * p.n_tiles + (l_on[j] ? tile : 0)) * p.k_blocks;
-        l_src[j] = p.wq + blk * 1024 + half * 512 + 16 * lane;
-        l_sc[j] = p.ws + blk * (GPB * 16) + g * (GPB * 2) + (GPB == 4 ? 4 * half : GPB == 2 ? 2 * half : 0);
+        const size_t blk = (static_cast<size_t>(it.e) * p.n_tiles + (l_on[j] ? tile : 0)) * p.k_blocks + l_b;
+        l_src[j] = p.wq + blk * 1024 + 16 * lane;
+        l_sc[j] = p.ws + blk * (GPB * 16) + g * (GPB * 2);
       }
     };
     auto fill = [&] {
@@ -189,81 +214,79 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         const uint32_t st = ring + l_stage * kStage;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t sd = st + 1024 + j * 128 * kSc + 4 * kSc * lane;
+          const uint32_t sd = st + 2048 + j * 128 * GPB + 4 * GPB * lane;
           if (l_on[j]) {
-            cp_async16(st + 512 * j + 16 * lane, l_src[j]);
-            cp_async_small<4 * kSc>(sd, l_sc[j]);
+            cp_async16(st + 1024 * j + 16 * lane, l_src[j]);
+            cp_async16(st + 1024 * j + 512 + 16 * lane, l_src[j] + 512);
+            if constexpr (GPB == 4)
+              cp_async16(sd, l_sc[j]);
+            else
+              cp_async_small<4 * GPB>(sd, l_sc[j]);
           } else {  // rows past the last tile: any codes, scale 0
 #pragma unroll
-            for (int i = 0; i < kSc; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sd + 4 * i), "r"(0) : "memory");
+            for (int i = 0; i < GPB; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sd + 4 * i), "r"(0) : "memory");
           }
-          l_src[j] += 1024;
-          l_sc[j] += GPB * 16;
+          l_src[j] += 1024 * kWdGroups;
+          l_sc[j] += GPB * 16 * kWdGroups;
         }
-        if (++l_stage == kWdRing) l_stage = 0;
-        if (++l_b == p.k_blocks) {
-          l_b = 0;
-          l_item += gridDim.x;
-          open();
-        }
+        if (++l_stage == kDepth) l_stage = 0;
+        l_b += kWdGroups;
+        if (l_b >= p.k_blocks) open();
       }
       cp_async_commit();
     };
     open();
 #pragma unroll
-    for (int d = 0; d < kWdRing - 1; ++d) fill();
-    // Steps of an item: 2 k_blocks, an even number like the ring's, so that each half always meets the
-    // same stages and waits for every use of them (a parity wait may not skip one).
-    int step = half;
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
-      for (int b = 0; b < p.k_blocks; ++b, step += 2) {
-        fill();  // the stage freed by the step before
-        cp_async_wait<kWdRing - 1>();
-        const uint32_t st = ring + u_stage * kStage;
-        if (++u_stage == kWdRing) u_stage = 0;
-        uint32_t r[2][16];
+    for (int d = 0; d < kDepth - 1; ++d) fill();
+    const int my_items = (items - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) /
+                         static_cast<int>(gridDim.x);
+    const int total = my_items * p.k_blocks;  // steps of this CTA
+    uint32_t phase = 1;
+    for (int step = group; step < total; step += kWdGroups, phase ^= 1) {
+      fill();  // the stage freed by the step before
+      cp_async_wait<kDepth - 1>();
+      const uint32_t st = ring + u_stage * kStage;
+      if (++u_stage == kDepth) u_stage = 0;
+      if (!warp_wait(&empty[group], phase, p.err, kErrTimeoutProducer)) break;
+      tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 q = lds128(st + 512 * j + 16 * lane);
-          const uint32_t sd = st + 1024 + j * 128 * kSc + 4 * kSc * lane;
+      for (int j = 0; j < 2; ++j) {
+        uint32_t sw[GPB];
+#pragma unroll
+        for (int i = 0; i < GPB; ++i) sw[i] = lds32(st + 2048 + j * 128 * GPB + 4 * GPB * lane + 4 * i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 64 columns
+          const uint4 q = lds128(st + 1024 * j + 512 * h + 16 * lane);
           const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+          uint32_t r[16];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {  // 32 columns
-            const uint32_t sw = lds32(sd + (kSc == 2 ? 4 * k : 0));
-            const __nv_bfloat162 sl = int4_scale2(sw, 0), sh = int4_scale2(sw, 1);
+            const uint32_t s = sw[(2 * h + k) * GPB / 4];
+            const __nv_bfloat162 sl = int4_scale2(s, 0), sh = int4_scale2(s, 1);
             const __nv_bfloat162 ml = int4_m24(sl), mh = int4_m24(sh);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              r[j][2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
-              r[j][2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
+              r[2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
+              r[2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
             }
           }
+          tmem_st_16x32(tmem + kWdTmemA + 64 * group + 32 * h + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16), r);
         }
-        const int s = step % kWdStages;
-        if (!mbar_wait(&empty[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t dst = tmem + kWdTmemA + 32 * s + (static_cast<uint32_t>(32 * quarter) << 16);
-        tmem_st_16x32(dst, r[0]);
-        tmem_st_16x32(dst + (16u << 16), r[1]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[s]);
       }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[group]);
     }
     cp_async_wait<0>();
-  } else if (warp < 12) {
+  } else if (warp < kWdDeqWarps + 4) {
     // ---------------------------------------------------------------- epilogue
     const int quarter = warp & 3;
     int li = 0;
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++li) {
       const WdItem it = item_of(i);
       const int buf = li & 1;
-      if (!mbar_wait(&tfull[buf], (li >> 1) & 1, p.err, kErrTimeoutEpilogue)) break;
+      if (!warp_wait(&tfull[buf], (li >> 1) & 1, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * kWdN + (static_cast<uint32_t>(32 * quarter) << 16);
       for (int c0 = 0; c0 < it.n; c0 += 32) {
@@ -305,7 +328,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[buf]);
     }
-  } else if (warp == 12) {
+  } else if (warp == kWdDeqWarps + 4) {
     // ---------------------------------------------------------------- TMA producer of x
     if (lane == 0) {
       const uint64_t policy = policy_evict_last();  // every row tile of the expert reads it
@@ -313,54 +336,67 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       bool ok = true;
       for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
         const WdItem it = item_of(i);
-        const int boxes = (it.n + 15) / 16;
-        for (int k = 0; k < 2 * p.k_blocks; ++k, ++step) {
+        // one box of 64 rows, or with few tokens boxes of 16 (rows past the item's are not used)
+        const int boxes = it.n > 32 ? 1 : (it.n + 15) / 16, rows = it.n > 32 ? 64 : 16;
+        const CUtensorMap* map = it.n > 32 ? &tmap_x64 : &tmap_x16;
+        for (int k = 0; k < p.k_blocks; ++k, ++step) {
           const int s = step % kWdStages;
           if (!mbar_wait(&empty[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full_b[s], boxes * 2048);
-          for (int r = 0; r < boxes; ++r)
-            tma_load_2d(smem + s * kWdBStage + r * 2048, &tmap_x, &full_b[s], k * 64, it.base + 16 * r, policy);
+          mbar_arrive_expect_tx(&full[s], 2 * boxes * rows * 128);
+          for (int h = 0; h < 2; ++h)
+            for (int r = 0; r < boxes; ++r)
+              tma_load_2d(smem + s * kWdBStage + h * kWdBHalf + r * 2048, map, &full[s], k * 128 + h * 64,
+                          it.base + 16 * r, policy);
         }
       }
       if (!ok)  // let the loads already issued land before shared memory goes away
         for (int j = max(0, step - kWdStages); j < step; ++j)
-          mbar_wait_ns(&full_b[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
+          mbar_wait_ns(&full[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
     }
-  } else if (lane == 0) {
+  } else {
     // ---------------------------------------------------------------- MMA issuer
+    // The whole warp walks the loop, so that the operands of the MMAs are known to be uniform; one
+    // elected lane issues.
     int step = 0, li = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
-      const WdItem it = item_of(i);
-      const uint32_t idesc = wd_idesc((it.n + 15) & ~15);
+      const int n = __shfl_sync(0xffffffffu, item_of(i).n, 0);
+      const uint32_t idesc = wd_idesc((n + 15) & ~15);
       const int buf = li & 1;
-      if (!mbar_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
-      for (int k = 0; k < 2 * p.k_blocks; ++k, ++step) {
+      if (!warp_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      for (int k = 0; k < p.k_blocks; ++k, ++step) {
         const int s = step % kWdStages;
-        const uint32_t ph = (step / kWdStages) & 1;
-        if (!mbar_wait(&full_b[s], ph, p.err, kErrTimeoutMma) || !mbar_wait(&full_a[s], ph, p.err, kErrTimeoutMma)) {
+        if (!warp_wait(&full[s], (step / kWdStages) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint64_t bd = sdesc_sw128(smem_u32(smem + s * kWdBStage));
+        const uint32_t d = tmem + buf * kWdN, a = tmem + kWdTmemA + 64 * s;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
-          tc_mma_bf16_ts(tmem + buf * kWdN, tmem + kWdTmemA + 32 * s + 8 * kk, bd + 2 * kk, idesc,
-                         (k | kk) != 0 ? 1u : 0u);
-        tc_commit(&empty[s]);
+          for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
+            tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
+                           (k | kk) != 0 ? 1u : 0u);
+          tc_commit(&empty[s]);
+        }
+        __syncwarp();
       }
-      if (ok) tc_commit(&tfull[buf]);
+      if (ok && elect_one()) tc_commit(&tfull[buf]);
+      __syncwarp();
     }
-    tc_commit(&drain);  // every MMA has finished before tensor memory is freed
-    mbar_wait_ns(&drain, 0, 100000000ull);
+    if (elect_one()) {
+      tc_commit(&drain);  // every MMA has finished before tensor memory is freed
+      mbar_wait_ns(&drain, 0, 100000000ull);
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == kWdDeqWarps + 5) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -419,27 +455,28 @@ __global__ void __launch_bounds__(256)
 }
 
 template <bool kUp, int GPB>
-cudaError_t launch_wide(const CUtensorMap& tx, const WdArgs& p, int grid, cudaStream_t st) {
+cudaError_t launch_wide(const CUtensorMap& t16, const CUtensorMap& t64, const WdArgs& p, int grid, cudaStream_t st) {
   const int smem = 1024 + kWdStages * kWdBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
   auto kern = wide_kernel<kUp, GPB>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kWdThreads, smem, st>>>(tx, p);
+  kern<<<grid, kWdThreads, smem, st>>>(t16, t64, p);
   return cudaGetLastError();
 }
 
 template <bool kUp>
 cudaError_t launch_wide(WdArgs p, const void* x, int ld, int n_entries, int group, cudaStream_t st) {
-  CUtensorMap tx;
-  if (!encode_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, static_cast<uint64_t>(ld),
-                      static_cast<uint64_t>(n_entries), 64, 16, true))
+  CUtensorMap t16, t64;
+  const uint64_t inner = static_cast<uint64_t>(ld), rows = static_cast<uint64_t>(n_entries);
+  if (!encode_tmap_2d(&t16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, inner, rows, 64, 16, true) ||
+      !encode_tmap_2d(&t64, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, inner, rows, 64, 64, true))
     return cudaErrorInvalidValue;
   const long long most = (n_entries / kWdN + static_cast<long long>(p.E < n_entries ? p.E : n_entries)) * p.m_tiles;
   const int sms = gemm_grid_sms();
   const int grid = most < sms ? static_cast<int>(most) : sms;
-  return group == 32   ? launch_wide<kUp, 4>(tx, p, grid, st)
-         : group == 64 ? launch_wide<kUp, 2>(tx, p, grid, st)
-                       : launch_wide<kUp, 1>(tx, p, grid, st);
+  return group == 32   ? launch_wide<kUp, 4>(t16, t64, p, grid, st)
+         : group == 64 ? launch_wide<kUp, 2>(t16, t64, p, grid, st)
+                       : launch_wide<kUp, 1>(t16, t64, p, grid, st);
 }
 
 }  // namespace
