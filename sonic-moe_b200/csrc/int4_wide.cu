@@ -1,6 +1,6 @@
 // Expert products with 4-bit weights for many tokens (format and layout: int4.cuh; few tokens: int4.cu).
 //
-// Grouped GEMMs on tcgen05 whose first operand is the weight: D[128 rows, tokens] = W[128, K] x[tokens, K]^T.
+// Grouped GEMMs on tcgen05 whose first operand is the weight: D[256 rows, tokens] = W[256, K] x[tokens, K]^T.
 // The codes go from global memory through shared memory into registers, become bf16 there (exact, scale
 // included) and are stored to tensor memory, from where the MMA reads its A operand; x comes through TMA
 // into 128-byte-swizzled shared memory.  Keeping A out of shared memory is what makes this bound by the
@@ -14,12 +14,15 @@
 // projection writes its intermediate in that order.
 //
 // Roles per CTA (704 threads, one CTA per SM):
-//   warps 0-15   dequantise: warp w stores rows 32 (w % 4) .. + 31 of every 4th step of 128 columns
-//   warps 16-19  epilogue: rows 32 (w % 4) .. of the accumulator (two accumulators of 64 columns)
+//   warps 0-15   dequantise; a group of 4 has one half of the rows and every other step of 128 columns,
+//                its warp w rows 32 (w % 4) .. + 31 of the half
+//   warps 16-19  epilogue: rows 32 (w % 4) .. of each accumulator (two of 64 columns, double buffered)
 //   warp 20      TMA producer of x,  warp 21  MMA issuer (and tensor memory allocation)
-// A step is as long as it is (8 MMAs of 16 columns) because the issuer's waits and commit cost some
-// hundred cycles whatever they guard; steps of 64 columns were bound by them.
-// Work items (expert, 128 rows, up to 64 of its tokens), rows fastest, static round robin; the items of
+// A step is as long as it is (8 MMAs of 16 columns for each half) because the issuer's waits and commit
+// cost some hundred cycles whatever they guard: steps of 64 columns were bound by them.  An item has 256
+// rows because x, which every row tile reads from L2, otherwise costs an SM twice the bytes of the
+// weights (64 tokens: 16 KB a step against 8 KB).
+// Work items (expert, 256 rows, up to 64 of its tokens), rows fastest, static round robin; the items of
 // an expert's token chunks follow each other, so their second reading of the weights is from L2.
 // Every wait is bounded; after a time-out the kernel records an error, drains and returns.
 #include "int4.cuh"
@@ -29,13 +32,13 @@ namespace smb {
 namespace {
 
 constexpr int kWdDeqWarps = 16;
-constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps make a step's 128 rows
+constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps store the 128 rows of half an item
 constexpr int kWdThreads = 32 * (kWdDeqWarps + 6);
-constexpr int kWdStages = 4;  // 128-column steps of x (shared memory) and of the weights (tensor memory)
+constexpr int kWdStages = 4;  // 128-column steps of x in shared memory; half steps of weights in tensor memory
 constexpr int kWdN = 64;      // tokens of an item at most
 constexpr int kWdBHalf = kWdN * 128;  // 64 columns of x
 constexpr int kWdBStage = 2 * kWdBHalf;
-constexpr uint32_t kWdTmemA = 256;  // accumulators at 0 and 64, A stages of 64 columns from here
+constexpr uint32_t kWdTmemA = 256;  // accumulators below (buffer 128, half 64), A stages of 64 columns from here
 static_assert(kWdStages == kWdGroups, "a group of dequantising warps owns a stage");
 
 template <int GPB>
@@ -109,7 +112,8 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmap_x16, const __grid_constant__ CUtensorMap tmap_x64,
                 const WdArgs p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kWdStages], empty[kWdStages], tfull[2], tempty[2], drain;
+  __shared__ uint64_t full_a[kWdGroups], empty_a[kWdGroups], full_b[kWdStages], empty_b[kWdStages], tfull[2], tempty[2],
+      drain;
   __shared__ uint32_t tmem_holder;
   __shared__ int32_t s_warp[kWdThreads / 32];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -120,8 +124,10 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < kWdStages; ++s) {
-      mbar_init(&full[s], 4 + 1);  // a group's warps and the producer of x
-      mbar_init(&empty[s], 1);
+      mbar_init(&full_a[s], 4);
+      mbar_init(&empty_a[s], 1);
+      mbar_init(&full_b[s], 1);
+      mbar_init(&empty_b[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
@@ -184,13 +190,13 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 
   if (warp < kWdDeqWarps) {
     // ---------------------------------------------------------------- dequantise
-    // Steps are numbered through all items of the CTA; group warp / 4 takes every 4th of them, and with
-    // them one stage.
+    // Steps are numbered through all items of the CTA; a group takes every other one, and one half of the
+    // rows, into the stage of tensor memory that is its own.
     constexpr int kStage = WdRing<GPB>::kStage, kDepth = WdRing<GPB>::kDepth;
     const Int4Magic magic;
-    const int quarter = warp & 3, group = warp >> 2, g = lane >> 2;
+    const int quarter = warp & 3, group = warp >> 2, half = group & 1, odd = group >> 1, g = lane >> 2;
     const uint32_t ring = smem_u32(rings) + warp * kDepth * kStage;
-    int l_item = blockIdx.x, l_b = group, l_stage = 0, u_stage = 0;
+    int l_item = blockIdx.x, l_b = odd, l_stage = 0, u_stage = 0;
     const uint8_t* l_src[2] = {};
     const __nv_bfloat16* l_sc[2] = {};
     bool l_on[2] = {};
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       const WdItem it = item_of(l_item);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int tile = it.mt * 8 + 2 * quarter + j;
+        const int tile = it.mt * 16 + 8 * half + 2 * quarter + j;
         l_on[j] = tile < p.n_tiles;
         const size_t blk = (static_cast<size_t>(it.e) * p.n_tiles + (l_on[j] ? tile : 0)) * p.k_blocks + l_b;
         l_src[j] = p.wq + blk * 1024 + 16 * lane;
@@ -226,11 +232,11 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 #pragma unroll
             for (int i = 0; i < GPB; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sd + 4 * i), "r"(0) : "memory");
           }
-          l_src[j] += 1024 * kWdGroups;
-          l_sc[j] += GPB * 16 * kWdGroups;
+          l_src[j] += 2 * 1024;
+          l_sc[j] += 2 * GPB * 16;
         }
         if (++l_stage == kDepth) l_stage = 0;
-        l_b += kWdGroups;
+        l_b += 2;
         if (l_b >= p.k_blocks) open();
       }
       cp_async_commit();
@@ -242,12 +248,12 @@ __global__ void __launch_bounds__(kWdThreads, 1)
                          static_cast<int>(gridDim.x);
     const int total = my_items * p.k_blocks;  // steps of this CTA
     uint32_t phase = 1;
-    for (int step = group; step < total; step += kWdGroups, phase ^= 1) {
+    for (int step = odd; step < total; step += 2, phase ^= 1) {
       fill();  // the stage freed by the step before
       cp_async_wait<kDepth - 1>();
       const uint32_t st = ring + u_stage * kStage;
       if (++u_stage == kDepth) u_stage = 0;
-      if (!warp_wait(&empty[group], phase, p.err, kErrTimeoutProducer)) break;
+      if (!warp_wait(&empty_a[group], phase, p.err, kErrTimeoutProducer)) break;
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[group]);
+      if (lane == 0) mbar_arrive(&full_a[group]);
     }
     cp_async_wait<0>();
   } else if (warp < kWdDeqWarps + 4) {
@@ -288,16 +294,17 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       const int buf = li & 1;
       if (!warp_wait(&tfull[buf], (li >> 1) & 1, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
-      const uint32_t acc = tmem + buf * kWdN + (static_cast<uint32_t>(32 * quarter) << 16);
-      for (int c0 = 0; c0 < it.n; c0 += 32) {
+      const int pieces = (it.n + 31) / 32;
+      for (int piece = 0; piece < 2 * pieces; ++piece) {  // half of the rows, 32 tokens
+        const int half = piece >= pieces, c0 = 32 * (piece - half * pieces);
         uint32_t v[32];
-        tmem_ld32(acc + c0, v);
+        tmem_ld32(tmem + buf * 128 + half * 64 + c0 + (static_cast<uint32_t>(32 * quarter) << 16), v);
         tmem_ld_wait();
         const int n = min(32, it.n - c0);
         if (kUp) {
           // even lanes hold gates, odd lanes the ups of the same output column: a pair finishes two tokens
           const bool odd = lane & 1;
-          const int col = it.mt * 64 + quarter * 16 + (lane >> 1);
+          const int col = it.mt * 128 + half * 64 + quarter * 16 + (lane >> 1);
           __nv_bfloat16* dst = p.a + static_cast<size_t>(it.base + c0) * p.a_ld + (col & ~31) + wd_place(col & 31);
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
             if (t < n) dst[static_cast<size_t>(t) * p.a_ld] = __float2bfloat16_rn(r);
           }
         } else {
-          const int row = it.mt * 128 + quarter * 32 + lane;
+          const int row = it.mt * 256 + half * 128 + quarter * 32 + lane;
           int f = 0;
           float sc = 0.0f;
           if (lane < n) {
@@ -341,20 +348,20 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         const CUtensorMap* map = it.n > 32 ? &tmap_x64 : &tmap_x16;
         for (int k = 0; k < p.k_blocks; ++k, ++step) {
           const int s = step % kWdStages;
-          if (!mbar_wait(&empty[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
+          if (!mbar_wait(&empty_b[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[s], 2 * boxes * rows * 128);
+          mbar_arrive_expect_tx(&full_b[s], 2 * boxes * rows * 128);
           for (int h = 0; h < 2; ++h)
             for (int r = 0; r < boxes; ++r)
-              tma_load_2d(smem + s * kWdBStage + h * kWdBHalf + r * 2048, map, &full[s], k * 128 + h * 64,
+              tma_load_2d(smem + s * kWdBStage + h * kWdBHalf + r * 2048, map, &full_b[s], k * 128 + h * 64,
                           it.base + 16 * r, policy);
         }
       }
       if (!ok)  // let the loads already issued land before shared memory goes away
         for (int j = max(0, step - kWdStages); j < step; ++j)
-          mbar_wait_ns(&full[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
+          mbar_wait_ns(&full_b[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
     }
   } else {
     // ---------------------------------------------------------------- MMA issuer
@@ -369,21 +376,29 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       if (!warp_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
         const int s = step % kWdStages;
-        if (!warp_wait(&full[s], (step / kWdStages) & 1, p.err, kErrTimeoutMma)) {
+        if (!warp_wait(&full_b[s], (step / kWdStages) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
-        tc_fence_after();
         const uint64_t bd = sdesc_sw128(smem_u32(smem + s * kWdBStage));
-        const uint32_t d = tmem + buf * kWdN, a = tmem + kWdTmemA + 64 * s;
-        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
-            tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
-                           (k | kk) != 0 ? 1u : 0u);
-          tc_commit(&empty[s]);
+        for (int half = 0; half < 2; ++half) {
+          const int g = 2 * (step & 1) + half;  // the group whose stage holds these weights
+          if (ok && !warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) ok = false;
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t d = tmem + buf * 128 + half * 64, a = tmem + kWdTmemA + 64 * g;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
+              tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
+                             (k | kk) != 0 ? 1u : 0u);
+            tc_commit(&empty_a[g]);
+            if (half == 1) tc_commit(&empty_b[s]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
       }
       if (ok && elect_one()) tc_commit(&tfull[buf]);
       __syncwarp();
@@ -498,7 +513,7 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   u.n_tiles = int4_row_tiles(u.N);
   u.k_blocks = int4_col_blocks(p.H);
   u.E = p.E;
-  u.m_tiles = int4_padded(p.I) / 64;  // the padding of the intermediate is written too (zeros)
+  u.m_tiles = int4_padded(p.I) / 128;  // 256 rows make 128 columns; the padding is written too (zeros)
   u.freq = p.freq;
   u.off = p.off;
   u.s_scatter = p.s_scatter;
@@ -513,7 +528,7 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   d.N = p.H;
   d.n_tiles = int4_row_tiles(d.N);
   d.k_blocks = int4_col_blocks(p.I);
-  d.m_tiles = ceil_div(d.N, 128);
+  d.m_tiles = ceil_div(d.N, 256);
   e = launch_wide<true>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st);
   if (e != cudaSuccess) return e;
   e = launch_wide<false>(d, p.a, u.a_ld, p.n_entries, p.group2, st);
