@@ -912,7 +912,7 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   p.group2 = w2_group;
   p.freq = expert_frequency;
   p.off = w.off;
-  p.s_scatter = w.s_scatter;
+  p.s_rev = w.s_rev;
   p.x_gather = w.x_gather;
   p.xs = w.xs;
   p.a = w.a;

@@ -13,15 +13,18 @@
 // place 8 i + 2 t + e.  x is gathered into expert order and permuted by wide_gather_kernel; the up
 // projection writes its intermediate in that order.
 //
-// Roles per CTA (704 threads, one CTA per SM):
+// Roles per CTA (736 threads, one CTA per SM):
 //   warps 0-15   dequantise; a group of 4 has one half of the rows and every other step of 128 columns,
 //                its warp w rows 32 (w % 4) .. + 31 of the half
 //   warps 16-19  epilogue: rows 32 (w % 4) .. of each accumulator (two of 64 columns, double buffered)
-//   warp 20      TMA producer of x,  warp 21  MMA issuer (and tensor memory allocation)
-// A step is as long as it is (8 MMAs of 16 columns for each half) because the issuer's waits and commit
-// cost some hundred cycles whatever they guard: steps of 64 columns were bound by them.  An item has 256
-// rows because x, which every row tile reads from L2, otherwise costs an SM twice the bytes of the
-// weights (64 tokens: 16 KB a step against 8 KB).
+//   warp 20      TMA producer of x
+//   warps 21-22  MMA issuers, one for each half of the rows (21 allocates tensor memory)
+// An issuer's waits and commits cost it some hundred cycles a step whatever they guard, as long as its 8
+// MMAs of 64 tokens take (32 cycles each).  So a step has 128 columns, the halves have an issuer each,
+// whose work the tensor core interleaves, and an issuer waits once and commits once a step: that x has
+// landed is waited for by the dequantising warps, before they announce their part.  An item has 256 rows
+// because x, which every row tile reads from L2, otherwise costs an SM twice the bytes of the weights
+// (64 tokens: 16 KB a step against 8 KB).
 // Work items (expert, 256 rows, up to 64 of its tokens), rows fastest, static round robin; the items of
 // an expert's token chunks follow each other, so their second reading of the weights is from L2.
 // Every wait is bounded; after a time-out the kernel records an error, drains and returns.
@@ -33,13 +36,12 @@ namespace {
 
 constexpr int kWdDeqWarps = 16;
 constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps store the 128 rows of half an item
-constexpr int kWdThreads = 32 * (kWdDeqWarps + 6);
+constexpr int kWdThreads = 32 * (kWdDeqWarps + 7);
 constexpr int kWdStages = 4;  // 128-column steps of x in shared memory; half steps of weights in tensor memory
 constexpr int kWdN = 64;      // tokens of an item at most
 constexpr int kWdBHalf = kWdN * 128;  // 64 columns of x
 constexpr int kWdBStage = 2 * kWdBHalf;
 constexpr uint32_t kWdTmemA = 256;  // accumulators below (buffer 128, half 64), A stages of 64 columns from here
-static_assert(kWdStages == kWdGroups, "a group of dequantising warps owns a stage");
 
 template <int GPB>
 struct WdRing {
@@ -55,11 +57,9 @@ struct WdArgs {
   int E, m_tiles;
   const int32_t* freq;
   const int32_t* off;
-  const int32_t* s_scatter;
-  const float* scores;
   __nv_bfloat16* a;  // up output [entries, a_ld], sorted order, permuted columns, zero beyond N / 2
   int a_ld;
-  float* y;  // down output [entries, N] by flat entry, times the score
+  float* y;  // down output [entries, N], sorted order
   int* err;
 };
 
@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmap_x16, const __grid_constant__ CUtensorMap tmap_x64,
                 const WdArgs p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_a[kWdGroups], empty_a[kWdGroups], full_b[kWdStages], empty_b[kWdStages], tfull[2], tempty[2],
-      drain;
+  // step n, half h: full_a[2 (n % 2) + h] both operands are there, done[h][n % kWdStages] the MMAs have read
+  // them; full_b[n % kWdStages] x is there
+  __shared__ uint64_t full_a[kWdGroups], full_b[kWdStages], done[2][kWdStages], tfull[2], tempty[2], drain[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int32_t s_warp[kWdThreads / 32];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -125,15 +126,15 @@ __global__ void __launch_bounds__(kWdThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < kWdStages; ++s) {
       mbar_init(&full_a[s], 4);
-      mbar_init(&empty_a[s], 1);
       mbar_init(&full_b[s], 1);
-      mbar_init(&empty_b[s], 1);
+      mbar_init(&done[0][s], 1);
+      mbar_init(&done[1][s], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&tfull[i], 1);
+      mbar_init(&tfull[i], 2);
       mbar_init(&tempty[i], 4);
+      mbar_init(&drain[i], 1);
     }
-    mbar_init(&drain, 1);
     fence_mbar_init();
     prefetch_tmap(&tmap_x16);
     prefetch_tmap(&tmap_x64);
@@ -247,13 +248,14 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     const int my_items = (items - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) /
                          static_cast<int>(gridDim.x);
     const int total = my_items * p.k_blocks;  // steps of this CTA
-    uint32_t phase = 1;
-    for (int step = odd; step < total; step += 2, phase ^= 1) {
+    for (int step = odd; step < total; step += 2) {
       fill();  // the stage freed by the step before
       cp_async_wait<kDepth - 1>();
       const uint32_t st = ring + u_stage * kStage;
       if (++u_stage == kDepth) u_stage = 0;
-      if (!warp_wait(&empty_a[group], phase, p.err, kErrTimeoutProducer)) break;
+      if (step >= 2 && !warp_wait(&done[half][(step - 2) % kWdStages], ((step - 2) / kWdStages) & 1, p.err,
+                                  kErrTimeoutProducer))
+        break;
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -281,6 +283,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       }
       tmem_st_wait();
       tc_fence_before();
+      if (quarter == 0 &&
+          !warp_wait(&full_b[step % kWdStages], (step / kWdStages) & 1, p.err, kErrTimeoutProducer))
+        break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&full_a[group]);
     }
@@ -305,29 +310,22 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           // even lanes hold gates, odd lanes the ups of the same output column: a pair finishes two tokens
           const bool odd = lane & 1;
           const int col = it.mt * 128 + half * 64 + quarter * 16 + (lane >> 1);
-          __nv_bfloat16* dst = p.a + static_cast<size_t>(it.base + c0) * p.a_ld + (col & ~31) + wd_place(col & 31);
+          __nv_bfloat16* dst =
+              p.a + static_cast<size_t>(it.base + c0 + (odd ? 1 : 0)) * p.a_ld + (col & ~31) + wd_place(col & 31);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
+          for (int c = 0; c < 32; c += 2, dst += 2 * p.a_ld) {
             const float v0 = __uint_as_float(v[c]), v1 = __uint_as_float(v[c + 1]);
             const float o = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
             const float r = odd ? silu_mul(o, v1) : silu_mul(v0, o);
-            const int t = c + (odd ? 1 : 0);
-            if (t < n) dst[static_cast<size_t>(t) * p.a_ld] = __float2bfloat16_rn(r);
+            if (c + (odd ? 1 : 0) < n) *dst = __float2bfloat16_rn(r);
           }
         } else {
           const int row = it.mt * 256 + half * 128 + quarter * 32 + lane;
-          int f = 0;
-          float sc = 0.0f;
-          if (lane < n) {
-            f = p.s_scatter[it.base + c0 + lane];
-            sc = p.scores[f];
-          }
+          float* dst = p.y + static_cast<size_t>(it.base + c0) * p.N + row;
+          if (row < p.N) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c >= n) break;
-            const int fc = __shfl_sync(0xffffffffu, f, c);
-            const float s = __shfl_sync(0xffffffffu, sc, c);
-            if (row < p.N) p.y[static_cast<size_t>(fc) * p.N + row] = s * __uint_as_float(v[c]);
+            for (int c = 0; c < 32; ++c, dst += p.N)
+              if (c < n) *dst = __uint_as_float(v[c]);
           }
         }
       }
@@ -348,7 +346,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         const CUtensorMap* map = it.n > 32 ? &tmap_x64 : &tmap_x16;
         for (int k = 0; k < p.k_blocks; ++k, ++step) {
           const int s = step % kWdStages;
-          if (!mbar_wait(&empty_b[s], ((step / kWdStages) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
+          const uint32_t ph = ((step / kWdStages) & 1) ^ 1;
+          if (!mbar_wait(&done[0][s], ph, p.err, kErrTimeoutProducer) ||
+              !mbar_wait(&done[1][s], ph, p.err, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -364,9 +364,10 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           mbar_wait_ns(&full_b[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
     }
   } else {
-    // ---------------------------------------------------------------- MMA issuer
+    // ---------------------------------------------------------------- MMA issuers
     // The whole warp walks the loop, so that the operands of the MMAs are known to be uniform; one
     // elected lane issues.
+    const int half = warp - (kWdDeqWarps + 5);
     int step = 0, li = 0;
     bool ok = true;
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
@@ -374,38 +375,32 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       const uint32_t idesc = wd_idesc((n + 15) & ~15);
       const int buf = li & 1;
       if (!warp_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 128 + half * 64;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
-        const int s = step % kWdStages;
-        if (!warp_wait(&full_b[s], (step / kWdStages) & 1, p.err, kErrTimeoutMma)) {
+        const int s = step % kWdStages, g = 2 * (step & 1) + half;
+        if (!warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
+        tc_fence_after();
         const uint64_t bd = sdesc_sw128(smem_u32(smem + s * kWdBStage));
+        const uint32_t a = tmem + kWdTmemA + 64 * g;
+        if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int g = 2 * (step & 1) + half;  // the group whose stage holds these weights
-          if (ok && !warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) ok = false;
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t d = tmem + buf * 128 + half * 64, a = tmem + kWdTmemA + 64 * g;
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
-              tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
-                             (k | kk) != 0 ? 1u : 0u);
-            tc_commit(&empty_a[g]);
-            if (half == 1) tc_commit(&empty_b[s]);
-          }
-          __syncwarp();
+          for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
+            tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
+                           (k | kk) != 0 ? 1u : 0u);
+          tc_commit(&done[half][s]);
         }
-        if (!ok) break;
+        __syncwarp();
       }
       if (ok && elect_one()) tc_commit(&tfull[buf]);
       __syncwarp();
     }
     if (elect_one()) {
-      tc_commit(&drain);  // every MMA has finished before tensor memory is freed
-      mbar_wait_ns(&drain, 0, 100000000ull);
+      tc_commit(&drain[half]);  // every MMA has finished before tensor memory is freed
+      mbar_wait_ns(&drain[half], 0, 100000000ull);
     }
     __syncwarp();
   }
@@ -418,52 +413,67 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 }
 
 // x rows in expert order with permuted columns: xs[pos][32 b + wd_place(k)] = x[token(pos)][32 b + k], zero
-// beyond K.  One thread per (position, block of 32 columns): a 4 x 4 transpose of column pairs.
+// beyond K.  Thread t of a quad reads columns 8 t .. + 7 of a block (4 pairs) and the quad transposes its
+// 4 x 4 pairs, so that both sides move whole 64-byte blocks per quad.
 __global__ void __launch_bounds__(256)
     wide_gather_kernel(const __nv_bfloat16* __restrict__ x, int T, int K, const int32_t* __restrict__ x_gather,
                        const int32_t* __restrict__ freq, const int32_t* __restrict__ off, int E, int blocks,
                        __nv_bfloat16* __restrict__ xs, int* err) {
   const int total = off[E - 1] + freq[E - 1];  // entries that were not rejected
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const int pos = static_cast<int>(i / blocks), b = static_cast<int>(i % blocks);
+  const int pos = blockIdx.x;
   if (pos >= total) return;
   const int tok = x_gather[pos];
   const bool ok = tok >= 0 && tok < T;
-  if (!ok && b == 0) atomicCAS(err, 0, kErrBadToken);
-  uint32_t w[4][4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    uint4 v = make_uint4(0, 0, 0, 0);
+  if (!ok && threadIdx.x == 0) atomicCAS(err, 0, kErrBadToken);
+  const int t = threadIdx.x & 3;
+  for (int b0 = 0; b0 < blocks; b0 += 64) {  // whole quads stay together for the shuffles
+    const int b = b0 + (threadIdx.x >> 2);
     const int k = 32 * b + 8 * t;
-    if (ok && k < K) v = *reinterpret_cast<const uint4*>(x + static_cast<size_t>(tok) * K + k);
-    w[t][0] = v.x;
-    w[t][1] = v.y;
-    w[t][2] = v.z;
-    w[t][3] = v.w;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (ok && k < K) v = __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(tok) * K + k));
+    // round 1: swap the 2 x 2 blocks between t and t ^ 2, round 2: within them between t and t ^ 1
+    const bool hi = t & 2, odd = t & 1;
+    const uint32_t s0 = __shfl_xor_sync(0xffffffffu, hi ? v.x : v.z, 2), s1 = __shfl_xor_sync(0xffffffffu, hi ? v.y : v.w, 2);
+    if (hi) {
+      v.x = s0;
+      v.y = s1;
+    } else {
+      v.z = s0;
+      v.w = s1;
+    }
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1), r1 = __shfl_xor_sync(0xffffffffu, odd ? v.z : v.w, 1);
+    if (odd) {
+      v.x = r0;
+      v.z = r1;
+    } else {
+      v.y = r0;
+      v.w = r1;
+    }
+    if (b < blocks) *reinterpret_cast<uint4*>(xs + (static_cast<size_t>(pos) * blocks + b) * 32 + 8 * t) = v;
   }
-  uint4* dst = reinterpret_cast<uint4*>(xs + (static_cast<size_t>(pos) * blocks + b) * 32);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) dst[c] = make_uint4(w[0][c], w[1][c], w[2][c], w[3][c]);
 }
 
-// out[t] = sum of the rows y[f] of t's entries, f in [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]),
-// in entry order, rounded once.  Entries whose expert or token was rejected have no row.
+// out[t] = sum over t's entries f, [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]), of scores[f] times
+// the row y[s_rev[f]], in entry order, rounded once.  Entries whose expert was rejected have no row.
 __global__ void __launch_bounds__(256)
-    int4_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
-                        const int32_t* __restrict__ experts, int E, __nv_bfloat16* __restrict__ out) {
+    wide_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
+                        const int32_t* __restrict__ experts, const float* __restrict__ scores,
+                        const int32_t* __restrict__ s_rev, int E, __nv_bfloat16* __restrict__ out) {
   const int t = blockIdx.y;
   const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
   if (c >= H) return;
   const int f0 = tok_off ? tok_off[t] : t * K, f1 = tok_off ? tok_off[t + 1] : (t + 1) * K;
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
   for (int f = f0; f < f1; ++f) {
     const int e = experts[f];
     if (e < 0 || e >= E) continue;
-    const float4 v = *reinterpret_cast<const float4*>(y + static_cast<size_t>(f) * H + c);
-    s.x += v.x;
-    s.y += v.y;
-    s.z += v.z;
-    s.w += v.w;
+    const float4 v = *reinterpret_cast<const float4*>(y + static_cast<size_t>(s_rev[f]) * H + c);
+    const float w = scores[f];
+    s.x = fmaf(w, v.x, s.x);
+    s.y = fmaf(w, v.y, s.y);
+    s.z = fmaf(w, v.z, s.z);
+    s.w = fmaf(w, v.w, s.w);
   }
   *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + c) =
       make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
@@ -500,8 +510,7 @@ int int4_padded(int K) { return int4_col_blocks(K) * 128; }
 
 cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   const int blocks = int4_padded(p.H) / 32;
-  const long long threads = static_cast<long long>(p.n_entries) * blocks;
-  wide_gather_kernel<<<static_cast<unsigned>((threads + 255) / 256), 256, 0, st>>>(
+  wide_gather_kernel<<<p.n_entries, 256, 0, st>>>(
       static_cast<const __nv_bfloat16*>(p.x), p.T, p.H, p.x_gather, p.freq, p.off, p.E, blocks,
       static_cast<__nv_bfloat16*>(p.xs), p.err);
   cudaError_t e = cudaGetLastError();
@@ -516,8 +525,6 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   u.m_tiles = int4_padded(p.I) / 128;  // 256 rows make 128 columns; the padding is written too (zeros)
   u.freq = p.freq;
   u.off = p.off;
-  u.s_scatter = p.s_scatter;
-  u.scores = p.scores;
   u.a = static_cast<__nv_bfloat16*>(p.a);
   u.a_ld = int4_padded(p.I);
   u.y = p.y;
@@ -535,9 +542,9 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   for (int t0 = 0; t0 < p.T; t0 += 32768) {  // grid.y limit
     const int n = p.T - t0 < 32768 ? p.T - t0 : 32768;
-    int4_combine_kernel<<<dim3(ceil_div(p.H, 1024), n), 256, 0, st>>>(
-        p.y + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K * p.H), n, p.H, p.K,
-        p.tok_off ? p.tok_off + t0 : nullptr, p.experts + (p.tok_off ? 0 : static_cast<size_t>(t0) * p.K), p.E,
+    const size_t f0 = p.tok_off ? 0 : static_cast<size_t>(t0) * p.K;
+    wide_combine_kernel<<<dim3(ceil_div(p.H, 1024), n), 256, 0, st>>>(
+        p.y, n, p.H, p.K, p.tok_off ? p.tok_off + t0 : nullptr, p.experts + f0, p.scores + f0, p.s_rev + f0, p.E,
         static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t0) * p.H);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;

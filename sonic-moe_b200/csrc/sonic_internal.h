@@ -111,7 +111,7 @@ struct Int4Args {
   // routing plan: counts, offsets and the entries in expert order
   int32_t* freq;
   const int32_t* off;
-  const int32_t* s_scatter;
+  const int32_t* s_rev;
   const int32_t* x_gather;
   void* xs;  // bf16 [entries, int4_padded(H)]
   void* a;   // bf16 [entries, int4_padded(I)] ([entries, I] with few tokens)
@@ -121,7 +121,7 @@ struct Int4Args {
 };
 int int4_padded(int K);
 cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st);
-// Few tokens: no routing plan (freq is written; off, s_scatter, x_gather, tok_off, xs, y unused; err may be null).
+// Few tokens: no routing plan (freq is written; off, s_rev, x_gather, tok_off, xs, y unused; err may be null).
 bool int4_small(int T, int n_entries);
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st);
 
