@@ -61,7 +61,7 @@ __device__ __forceinline__ __nv_bfloat162 int4_m24(__nv_bfloat162 s) {
   return __hmul2(s, __floats2bfloat162_rn(-24.0f, -24.0f));
 }
 
-__device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+__device__ __forceinline__ float silu_mul(float gate, float up) { return __fdividef(gate, 1.0f + __expf(-gate)) * up; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

@@ -37,7 +37,7 @@ namespace {
 constexpr int kWdDeqWarps = 16;
 constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps store the 128 rows of half an item
 constexpr int kWdThreads = 32 * (kWdDeqWarps + 7);
-constexpr int kWdStages = 4;  // 128-column steps of x in shared memory; half steps of weights in tensor memory
+constexpr int kWdStages = 6;  // 128-column steps of x in shared memory
 constexpr int kWdN = 64;      // tokens of an item at most
 constexpr int kWdBHalf = kWdN * 128;  // 64 columns of x
 constexpr int kWdBStage = 2 * kWdBHalf;
@@ -46,7 +46,7 @@ constexpr uint32_t kWdTmemA = 256;  // accumulators below (buffer 128, half 64),
 template <int GPB>
 struct WdRing {
   static constexpr int kStage = 2 * (1024 + 128 * GPB);  // a step of 2 row tiles, GPB scale words a lane
-  static constexpr int kDepth = GPB == 4 ? 3 : 4;        // steps of codes in flight per dequantising warp
+  static constexpr int kDepth = GPB == 4 ? 2 : 3;        // steps of codes in flight per dequantising warp
   static constexpr int kBytes = kWdDeqWarps * kDepth * kStage;
 };
 
@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(kWdThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
+    for (int g = 0; g < kWdGroups; ++g) mbar_init(&full_a[g], 4);
     for (int s = 0; s < kWdStages; ++s) {
-      mbar_init(&full_a[s], 4);
       mbar_init(&full_b[s], 1);
       mbar_init(&done[0][s], 1);
       mbar_init(&done[1][s], 1);
@@ -248,25 +248,21 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     const int my_items = (items - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) /
                          static_cast<int>(gridDim.x);
     const int total = my_items * p.k_blocks;  // steps of this CTA
+    bool ok = true;
     for (int step = odd; step < total; step += 2) {
       fill();  // the stage freed by the step before
       cp_async_wait<kDepth - 1>();
       const uint32_t st = ring + u_stage * kStage;
       if (++u_stage == kDepth) u_stage = 0;
-      if (step >= 2 && !warp_wait(&done[half][(step - 2) % kWdStages], ((step - 2) / kWdStages) & 1, p.err,
-                                  kErrTimeoutProducer))
-        break;
-      tc_fence_after();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint32_t sw[GPB];
+        uint32_t sw[GPB], r[2][16];
 #pragma unroll
         for (int i = 0; i < GPB; ++i) sw[i] = lds32(st + 2048 + j * 128 * GPB + 4 * GPB * lane + 4 * i);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 64 columns
           const uint4 q = lds128(st + 1024 * j + 512 * h + 16 * lane);
           const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-          uint32_t r[16];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {  // 32 columns
             const uint32_t s = sw[(2 * h + k) * GPB / 4];
@@ -274,13 +270,24 @@ __global__ void __launch_bounds__(kWdThreads, 1)
             const __nv_bfloat162 ml = int4_m24(sl), mh = int4_m24(sh);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              r[2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
-              r[2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
+              r[h][2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
+              r[h][2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
             }
           }
-          tmem_st_16x32(tmem + kWdTmemA + 64 * group + 32 * h + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16), r);
         }
+        if (j == 0) {  // the first tile is ready while the MMAs still read the stage
+          if (step >= 2 && !warp_wait(&done[half][(step - 2) % kWdStages], ((step - 2) / kWdStages) & 1, p.err,
+                                      kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        const uint32_t dst = tmem + kWdTmemA + 64 * group + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16);
+        tmem_st_16x32(dst, r[0]);
+        tmem_st_16x32(dst + 32, r[1]);
       }
+      if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       if (quarter == 0 &&
@@ -341,9 +348,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       bool ok = true;
       for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
         const WdItem it = item_of(i);
-        // one box of 64 rows, or with few tokens boxes of 16 (rows past the item's are not used)
-        const int boxes = it.n > 32 ? 1 : (it.n + 15) / 16, rows = it.n > 32 ? 64 : 16;
-        const CUtensorMap* map = it.n > 32 ? &tmap_x64 : &tmap_x16;
+        // one box of 64 rows, or with fewer tokens boxes of 16 (rows past the item's are not used)
+        const int boxes = it.n > 48 ? 1 : (it.n + 15) / 16, rows = it.n > 48 ? 64 : 16;
+        const CUtensorMap* map = it.n > 48 ? &tmap_x64 : &tmap_x16;
         for (int k = 0; k < p.k_blocks; ++k, ++step) {
           const int s = step % kWdStages;
           const uint32_t ph = ((step / kWdStages) & 1) ^ 1;
