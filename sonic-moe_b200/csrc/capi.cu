@@ -921,6 +921,12 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   p.err = err;
   if (int4_small(T, n_entries)) return cuda_status(launch_int4_small(p, st), "moe_int4_forward");
   p.err = err ? err : w.err;
+  if (int4_plan_fits(n_entries, E)) {
+    cudaError_t e = launch_int4_plan(expert_indices, token_indices, n_entries, T, K, E, expert_frequency, w.off, w.s_rev,
+                                     w.x_gather, w.tok_off, p.err, !err, st);
+    if (e == cudaSuccess) e = launch_int4_wide(p, st);
+    return cuda_status(e, "moe_int4_forward");
+  }
   cudaError_t e = cudaSuccess;
   if (!err) e = cudaMemsetAsync(w.err, 0, sizeof(int32_t), st);
   const int per_tile = token_indices ? 1024 : kTileTokens * K;

@@ -315,8 +315,6 @@ __device__ __forceinline__ uint4 ld_plain(const void* p) {
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // A warp's ring: kDepth stages of one column block of MT row tiles, lane l's 16-byte piece h of tile m at
 // (2 m + h) * 512 + 16 l, then its scales (GPB words) at MT * 1024 + m * 128 GPB + 4 GPB l.
@@ -764,21 +762,7 @@ cudaError_t launch_small_down(SmallArgs p, cudaStream_t st) {
   auto kern = small_down_kernel<MT, NT, GPB>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles * cluster);
-  cfg.blockDim = dim3(kMvThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<const SmallArgs>(p));
+  return launch_dependent(kern, dim3(tiles * cluster), kMvThreads, smem, cluster, st, p);
 }
 
 template <int MT, int NT>
@@ -794,7 +778,7 @@ cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int
 
 }  // namespace
 
-bool int4_small(int T, int n_entries) { return T <= 64 && n_entries <= kSmMaxEntries; }
+bool int4_small(int T, int n_entries) { return T <= 8 && n_entries <= kSmMaxEntries; }
 
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st) {
   SmallArgs u{};

@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     tmem_alloc(&tmem_holder, 512);
     tmem_relinquish();
   }
+  pdl_launch();
+  pdl_wait();
   {  // chunks of kWdN tokens per expert, exclusive prefix
     const int per = (p.E + kWdThreads - 1) / kWdThreads;
     const int e0 = min(p.E, tid * per), e1 = min(p.E, e0 + per);
@@ -419,6 +421,72 @@ __global__ void __launch_bounds__(kWdThreads, 1)
   }
 }
 
+// Routing plan of few entries (kPlanMaxEntries) and experts (kPlanMaxExperts) in one CTA: counts, offsets,
+// an expert order (s_rev: place of an entry, x_gather: token of a place) and, for explicit lists, the
+// entries of each token.  The order of an expert's entries is that of shared-memory atomics: it decides
+// which column of a product an entry takes, and no column's value depends on that.  (For more entries,
+// the tiled kernels of router.cu.)
+constexpr int kPlanMaxEntries = 32768, kPlanMaxExperts = 1024;
+
+__global__ void __launch_bounds__(1024)
+    wide_plan_kernel(const int32_t* __restrict__ experts, const int32_t* __restrict__ tokens, int n, int T, int K, int E,
+                     int32_t* __restrict__ freq, int32_t* __restrict__ off, int32_t* __restrict__ s_rev,
+                     int32_t* __restrict__ x_gather, int32_t* __restrict__ tok_off, int* err, int clear_err) {
+  __shared__ int32_t s_cnt[kPlanMaxExperts], s_sum[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch();
+  s_cnt[tid] = 0;
+  if (clear_err && tid == 0) *err = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int f = tid; f < n; f += 1024) {
+    const int e = experts[f];
+    if (e >= 0 && e < E)
+      s_rev[f] = atomicAdd(&s_cnt[e], 1);
+    else
+      atomicCAS(err, 0, kErrBadExpert);
+  }
+  __syncthreads();
+  const int count = s_cnt[tid];  // zero beyond E
+  int inc = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) s_sum[warp] = inc;
+  __syncthreads();
+  int base = inc - count;
+  for (int w = 0; w < warp; ++w) base += s_sum[w];
+  s_cnt[tid] = base;
+  if (tid < E) {
+    freq[tid] = count;
+    off[tid] = base;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int f = tid; f < n; f += 1024) {
+    const int e = experts[f];
+    if (e >= 0 && e < E) {
+      const int pos = s_cnt[e] + s_rev[f];
+      s_rev[f] = pos;
+      x_gather[pos] = tokens ? tokens[f] : f / K;
+    }
+  }
+  if (tokens)
+    for (int t = tid; t <= T; t += 1024) {  // first entry of token t (the list is sorted)
+      int lo = 0, hi = n;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (tokens[mid] < t)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      tok_off[t] = lo;
+    }
+}
+
 // x rows in expert order with permuted columns: xs[pos][32 b + wd_place(k)] = x[token(pos)][32 b + k], zero
 // beyond K.  Thread t of a quad reads columns 8 t .. + 7 of a block (4 pairs) and the quad transposes its
 // 4 x 4 pairs, so that both sides move whole 64-byte blocks per quad.
@@ -426,6 +494,8 @@ __global__ void __launch_bounds__(256)
     wide_gather_kernel(const __nv_bfloat16* __restrict__ x, int T, int K, const int32_t* __restrict__ x_gather,
                        const int32_t* __restrict__ freq, const int32_t* __restrict__ off, int E, int blocks,
                        __nv_bfloat16* __restrict__ xs, int* err) {
+  pdl_launch();
+  pdl_wait();
   const int total = off[E - 1] + freq[E - 1];  // entries that were not rejected
   const int pos = blockIdx.x;
   if (pos >= total) return;
@@ -466,6 +536,7 @@ __global__ void __launch_bounds__(256)
     wide_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
                         const int32_t* __restrict__ experts, const float* __restrict__ scores,
                         const int32_t* __restrict__ s_rev, int E, __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
   const int t = blockIdx.y;
   const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
   if (c >= H) return;
@@ -492,8 +563,7 @@ cudaError_t launch_wide(const CUtensorMap& t16, const CUtensorMap& t64, const Wd
   auto kern = wide_kernel<kUp, GPB>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kWdThreads, smem, st>>>(t16, t64, p);
-  return cudaGetLastError();
+  return launch_dependent(kern, dim3(grid), kWdThreads, smem, 1, st, t16, t64, p);
 }
 
 template <bool kUp>
@@ -515,12 +585,21 @@ cudaError_t launch_wide(WdArgs p, const void* x, int ld, int n_entries, int grou
 
 int int4_padded(int K) { return int4_col_blocks(K) * 128; }
 
+bool int4_plan_fits(int n_entries, int E) { return n_entries <= kPlanMaxEntries && E <= kPlanMaxExperts; }
+
+cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int n, int T, int K, int E, int32_t* freq,
+                             int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
+                             bool clear_err, cudaStream_t st) {
+  wide_plan_kernel<<<1, 1024, 0, st>>>(experts, tokens, n, T, K, E, freq, off, s_rev, x_gather, tok_off, err,
+                                          clear_err);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   const int blocks = int4_padded(p.H) / 32;
-  wide_gather_kernel<<<p.n_entries, 256, 0, st>>>(
-      static_cast<const __nv_bfloat16*>(p.x), p.T, p.H, p.x_gather, p.freq, p.off, p.E, blocks,
-      static_cast<__nv_bfloat16*>(p.xs), p.err);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_dependent(
+      wide_gather_kernel, dim3(p.n_entries), 256, 0, 1, st, static_cast<const __nv_bfloat16*>(p.x), p.T, p.H,
+      p.x_gather, p.freq, p.off, p.E, blocks, static_cast<__nv_bfloat16*>(p.xs), p.err);
   if (e != cudaSuccess) return e;
   WdArgs u{};
   u.wq = p.w1q;
@@ -550,10 +629,10 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   for (int t0 = 0; t0 < p.T; t0 += 32768) {  // grid.y limit
     const int n = p.T - t0 < 32768 ? p.T - t0 : 32768;
     const size_t f0 = p.tok_off ? 0 : static_cast<size_t>(t0) * p.K;
-    wide_combine_kernel<<<dim3(ceil_div(p.H, 1024), n), 256, 0, st>>>(
-        p.y, n, p.H, p.K, p.tok_off ? p.tok_off + t0 : nullptr, p.experts + f0, p.scores + f0, p.s_rev + f0, p.E,
+    e = launch_dependent(
+        wide_combine_kernel, dim3(ceil_div(p.H, 1024), n), 256, 0, 1, st, p.y, n, p.H, p.K,
+        p.tok_off ? p.tok_off + t0 : nullptr, p.experts + f0, p.scores + f0, p.s_rev + f0, p.E,
         static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t0) * p.H);
-    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

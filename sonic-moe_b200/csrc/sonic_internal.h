@@ -121,6 +121,11 @@ struct Int4Args {
 };
 int int4_padded(int K);
 cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st);
+// The routing plan of launch_int4_wide in one launch, for sizes that fit; clear_err zeroes *err first.
+bool int4_plan_fits(int n_entries, int E);
+cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int n, int T, int K, int E, int32_t* freq,
+                             int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
+                             bool clear_err, cudaStream_t st);
 // Few tokens: no routing plan (freq is written; off, s_rev, x_gather, tok_off, xs, y unused; err may be null).
 bool int4_small(int T, int n_entries);
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st);

@@ -92,6 +92,8 @@ LAYER = [
     (100, 512, 1032, 4, 2, 128, True, 0.0),
     (300, 640, 128, 16, 6, 64, False, 1.2),
     (1000, 256, 256, 7, 3, 128, False, 1.2),
+    (40, 64, 24, 1100, 4, 32, False, 0.0),  # more experts, more entries than the one-launch routing plan takes
+    (5000, 64, 16, 9, 7, 64, True, 1.2),
 ]
 
 
