@@ -16,7 +16,7 @@
 // Roles per CTA (736 threads, one CTA per SM):
 //   warps 0-15   dequantise; a group of 4 has one half of the rows and every other step of 128 columns,
 //                its warp w rows 32 (w % 4) .. + 31 of the half
-//   warps 16-19  epilogue: rows 32 (w % 4) .. of each accumulator (two of 64 columns, double buffered)
+//   warps 16-19  epilogue: rows 32 (w % 4) .. of the accumulators of the two halves
 //   warp 20      TMA producer of x
 //   warps 21-22  MMA issuers, one for each half of the rows (21 allocates tensor memory)
 // An issuer's waits and commits cost it some hundred cycles a step whatever they guard, as long as its 8
@@ -25,8 +25,10 @@
 // landed is waited for by the dequantising warps, before they announce their part.  An item has 256 rows
 // because x, which every row tile reads from L2, otherwise costs an SM twice the bytes of the weights
 // (64 tokens: 16 KB a step against 8 KB).
-// Work items (expert, 256 rows, up to 64 of its tokens), rows fastest, static round robin; the items of
-// an expert's token chunks follow each other, so their second reading of the weights is from L2.
+// Work items (expert, 256 rows, up to kN of its tokens), rows fastest, static round robin; the items of
+// an expert's token chunks follow each other, so their second reading of the weights is from L2.  kN is
+// 64 with double-buffered accumulators (the epilogue overlaps the next item), or 128 with single ones,
+// which halves the dequantising per token.
 // Every wait is bounded; after a time-out the kernel records an error, drains and returns.
 #include "int4.cuh"
 
@@ -37,11 +39,16 @@ namespace {
 constexpr int kWdDeqWarps = 16;
 constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps store the 128 rows of half an item
 constexpr int kWdThreads = 32 * (kWdDeqWarps + 7);
-constexpr int kWdStages = 6;  // 128-column steps of x in shared memory
-constexpr int kWdN = 64;      // tokens of an item at most
-constexpr int kWdBHalf = kWdN * 128;  // 64 columns of x
-constexpr int kWdBStage = 2 * kWdBHalf;
-constexpr uint32_t kWdTmemA = 256;  // accumulators below (buffer 128, half 64), A stages of 64 columns from here
+constexpr uint32_t kWdTmemA = 256;  // accumulators below, A stages of 64 columns from here
+
+template <int kN>  // tokens of an item at most
+struct WdShape {
+  static constexpr int kBufs = 128 / kN;  // accumulator buffers of two halves of kN columns
+  static constexpr int kBHalf = kN * 128;  // 64 columns of x
+  static constexpr int kBStage = 2 * kBHalf;
+  static constexpr int kStages = 98304 / kBStage;  // 128-column steps of x in shared memory
+  static_assert(kBufs * 2 * kN == 256, "accumulators fill the columns below kWdTmemA");
+};
 
 template <int GPB>
 struct WdRing {
@@ -101,40 +108,43 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, where));
 }
 
-// Tokens of one of an expert's ceil(n / kWdN) chunks: equal shares, whole 16s but for the last.
+// Tokens of one of an expert's ceil(n / kN) chunks: equal shares, whole 16s but for the last.
 __device__ __forceinline__ int wd_share(int n, int chunks) { return ((n + chunks - 1) / chunks + 15) & ~15; }
 
 // Place of column k (< 32) of a block of 32 in the permuted order.
 __device__ __forceinline__ int wd_place(int k) { return 8 * ((k >> 1) & 3) + 2 * (k >> 3) + (k & 1); }
 
-template <bool kUp, int GPB>
+template <bool kUp, int kN, int GPB>
 __global__ void __launch_bounds__(kWdThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmap_x16, const __grid_constant__ CUtensorMap tmap_x64,
                 const WdArgs p) {
+  using Shape = WdShape<kN>;
+  constexpr int kStages = Shape::kStages, kBufs = Shape::kBufs;
   extern __shared__ uint8_t smem_raw[];
-  // step n, half h: full_a[2 (n % 2) + h] both operands are there, done[h][n % kWdStages] the MMAs have read
-  // them; full_b[n % kWdStages] x is there
-  __shared__ uint64_t full_a[kWdGroups], full_b[kWdStages], done[2][kWdStages], tfull[2], tempty[2], drain[2];
+  // step n, half h: full_a[2 (n % 2) + h] both operands are there, done[h][n % kStages] the MMAs have read
+  // them; full_b[n % kStages] x is there
+  __shared__ uint64_t full_a[kWdGroups], full_b[kStages], done[2][kStages], tfull[kBufs], tempty[kBufs], drain[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int32_t s_warp[kWdThreads / 32];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  uint8_t* rings = smem + kWdStages * kWdBStage;
+  uint8_t* rings = smem + kStages * Shape::kBStage;
   int32_t* pre = reinterpret_cast<int32_t*>(rings + WdRing<GPB>::kBytes);  // [E + 1] chunks before each expert
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int g = 0; g < kWdGroups; ++g) mbar_init(&full_a[g], 4);
-    for (int s = 0; s < kWdStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_b[s], 1);
       mbar_init(&done[0][s], 1);
       mbar_init(&done[1][s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBufs; ++i) {
       mbar_init(&tfull[i], 2);
       mbar_init(&tempty[i], 4);
-      mbar_init(&drain[i], 1);
     }
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_mbar_init();
     prefetch_tmap(&tmap_x16);
     prefetch_tmap(&tmap_x64);
@@ -145,11 +155,11 @@ __global__ void __launch_bounds__(kWdThreads, 1)
   }
   pdl_launch();
   pdl_wait();
-  {  // chunks of kWdN tokens per expert, exclusive prefix
+  {  // chunks of kN tokens per expert, exclusive prefix
     const int per = (p.E + kWdThreads - 1) / kWdThreads;
     const int e0 = min(p.E, tid * per), e1 = min(p.E, e0 + per);
     int c = 0;
-    for (int e = e0; e < e1; ++e) c += (p.freq[e] + kWdN - 1) / kWdN;
+    for (int e = e0; e < e1; ++e) c += (p.freq[e] + kN - 1) / kN;
     int inc = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -162,7 +172,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     for (int w = 0; w < warp; ++w) run += s_warp[w];
     for (int e = e0; e < e1; ++e) {
       pre[e] = run;
-      run += (p.freq[e] + kWdN - 1) / kWdN;
+      run += (p.freq[e] + kN - 1) / kN;
     }
     if (tid == kWdThreads - 1) pre[p.E] = run;
   }
@@ -278,7 +288,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           }
         }
         if (j == 0) {  // the first tile is ready while the MMAs still read the stage
-          if (step >= 2 && !warp_wait(&done[half][(step - 2) % kWdStages], ((step - 2) / kWdStages) & 1, p.err,
+          if (step >= 2 && !warp_wait(&done[half][(step - 2) % kStages], ((step - 2) / kStages) & 1, p.err,
                                       kErrTimeoutProducer)) {
             ok = false;
             break;
@@ -293,7 +303,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       if (quarter == 0 &&
-          !warp_wait(&full_b[step % kWdStages], (step / kWdStages) & 1, p.err, kErrTimeoutProducer))
+          !warp_wait(&full_b[step % kStages], (step / kStages) & 1, p.err, kErrTimeoutProducer))
         break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&full_a[group]);
@@ -305,14 +315,14 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     int li = 0;
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++li) {
       const WdItem it = item_of(i);
-      const int buf = li & 1;
-      if (!warp_wait(&tfull[buf], (li >> 1) & 1, p.err, kErrTimeoutEpilogue)) break;
+      const int buf = li % kBufs;
+      if (!warp_wait(&tfull[buf], (li / kBufs) & 1, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const int pieces = (it.n + 31) / 32;
       for (int piece = 0; piece < 2 * pieces; ++piece) {  // half of the rows, 32 tokens
         const int half = piece >= pieces, c0 = 32 * (piece - half * pieces);
         uint32_t v[32];
-        tmem_ld32(tmem + buf * 128 + half * 64 + c0 + (static_cast<uint32_t>(32 * quarter) << 16), v);
+        tmem_ld32(tmem + (2 * buf + half) * kN + c0 + (static_cast<uint32_t>(32 * quarter) << 16), v);
         tmem_ld_wait();
         const int n = min(32, it.n - c0);
         if (kUp) {
@@ -350,12 +360,12 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       bool ok = true;
       for (int i = blockIdx.x; ok && i < items; i += gridDim.x) {
         const WdItem it = item_of(i);
-        // one box of 64 rows, or with fewer tokens boxes of 16 (rows past the item's are not used)
-        const int boxes = it.n > 48 ? 1 : (it.n + 15) / 16, rows = it.n > 48 ? 64 : 16;
+        // boxes of 64 rows, or with fewer tokens of 16 (rows past the item's are not used)
+        const int rows = it.n > 48 ? 64 : 16, boxes = (it.n + rows - 1) / rows;
         const CUtensorMap* map = it.n > 48 ? &tmap_x64 : &tmap_x16;
         for (int k = 0; k < p.k_blocks; ++k, ++step) {
-          const int s = step % kWdStages;
-          const uint32_t ph = ((step / kWdStages) & 1) ^ 1;
+          const int s = step % kStages;
+          const uint32_t ph = ((step / kStages) & 1) ^ 1;
           if (!mbar_wait(&done[0][s], ph, p.err, kErrTimeoutProducer) ||
               !mbar_wait(&done[1][s], ph, p.err, kErrTimeoutProducer)) {
             ok = false;
@@ -364,13 +374,13 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           mbar_arrive_expect_tx(&full_b[s], 2 * boxes * rows * 128);
           for (int h = 0; h < 2; ++h)
             for (int r = 0; r < boxes; ++r)
-              tma_load_2d(smem + s * kWdBStage + h * kWdBHalf + r * 2048, map, &full_b[s], k * 128 + h * 64,
-                          it.base + 16 * r, policy);
+              tma_load_2d(smem + s * Shape::kBStage + h * Shape::kBHalf + r * rows * 128, map, &full_b[s],
+                          k * 128 + h * 64, it.base + rows * r, policy);
         }
       }
       if (!ok)  // let the loads already issued land before shared memory goes away
-        for (int j = max(0, step - kWdStages); j < step; ++j)
-          mbar_wait_ns(&full_b[j % kWdStages], (j / kWdStages) & 1, 50000000ull);
+        for (int j = max(0, step - kStages); j < step; ++j)
+          mbar_wait_ns(&full_b[j % kStages], (j / kStages) & 1, 50000000ull);
     }
   } else {
     // ---------------------------------------------------------------- MMA issuers
@@ -382,23 +392,23 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
       const int n = __shfl_sync(0xffffffffu, item_of(i).n, 0);
       const uint32_t idesc = wd_idesc((n + 15) & ~15);
-      const int buf = li & 1;
-      if (!warp_wait(&tempty[buf], ((li >> 1) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      const int buf = li % kBufs;
+      if (!warp_wait(&tempty[buf], ((li / kBufs) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
       tc_fence_after();
-      const uint32_t d = tmem + buf * 128 + half * 64;
+      const uint32_t d = tmem + (2 * buf + half) * kN;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
-        const int s = step % kWdStages, g = 2 * (step & 1) + half;
+        const int s = step % kStages, g = 2 * (step & 1) + half;
         if (!warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint64_t bd = sdesc_sw128(smem_u32(smem + s * kWdBStage));
+        const uint64_t bd = sdesc_sw128(smem_u32(smem + s * Shape::kBStage));
         const uint32_t a = tmem + kWdTmemA + 64 * g;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
-            tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (kWdBHalf >> 4) + 2 * (kk & 3), idesc,
+            tc_mma_bf16_ts(d, a + 8 * kk, bd + (kk >> 2) * (Shape::kBHalf >> 4) + 2 * (kk & 3), idesc,
                            (k | kk) != 0 ? 1u : 0u);
           tc_commit(&done[half][s]);
         }
@@ -557,28 +567,28 @@ __global__ void __launch_bounds__(256)
       make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
 }
 
-template <bool kUp, int GPB>
+template <bool kUp, int kN, int GPB>
 cudaError_t launch_wide(const CUtensorMap& t16, const CUtensorMap& t64, const WdArgs& p, int grid, cudaStream_t st) {
-  const int smem = 1024 + kWdStages * kWdBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
-  auto kern = wide_kernel<kUp, GPB>;
+  const int smem = 1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
+  auto kern = wide_kernel<kUp, kN, GPB>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   return launch_dependent(kern, dim3(grid), kWdThreads, smem, 1, st, t16, t64, p);
 }
 
-template <bool kUp>
+template <bool kUp, int kN>
 cudaError_t launch_wide(WdArgs p, const void* x, int ld, int n_entries, int group, cudaStream_t st) {
   CUtensorMap t16, t64;
   const uint64_t inner = static_cast<uint64_t>(ld), rows = static_cast<uint64_t>(n_entries);
   if (!encode_tmap_2d(&t16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, inner, rows, 64, 16, true) ||
       !encode_tmap_2d(&t64, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, inner, rows, 64, 64, true))
     return cudaErrorInvalidValue;
-  const long long most = (n_entries / kWdN + static_cast<long long>(p.E < n_entries ? p.E : n_entries)) * p.m_tiles;
+  const long long most = (n_entries / kN + static_cast<long long>(p.E < n_entries ? p.E : n_entries)) * p.m_tiles;
   const int sms = gemm_grid_sms();
   const int grid = most < sms ? static_cast<int>(most) : sms;
-  return group == 32   ? launch_wide<kUp, 4>(t16, t64, p, grid, st)
-         : group == 64 ? launch_wide<kUp, 2>(t16, t64, p, grid, st)
-                       : launch_wide<kUp, 1>(t16, t64, p, grid, st);
+  return group == 32   ? launch_wide<kUp, kN, 4>(t16, t64, p, grid, st)
+         : group == 64 ? launch_wide<kUp, kN, 2>(t16, t64, p, grid, st)
+                       : launch_wide<kUp, kN, 1>(t16, t64, p, grid, st);
 }
 
 }  // namespace
@@ -622,9 +632,13 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   d.n_tiles = int4_row_tiles(d.N);
   d.k_blocks = int4_col_blocks(p.I);
   d.m_tiles = ceil_div(d.N, 256);
-  e = launch_wide<true>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st);
+  // items of 128 tokens once the experts have 64 on average
+  const bool many = p.n_entries >= 64 * p.E;
+  e = many ? launch_wide<true, 128>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st)
+           : launch_wide<true, 64>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st);
   if (e != cudaSuccess) return e;
-  e = launch_wide<false>(d, p.a, u.a_ld, p.n_entries, p.group2, st);
+  e = many ? launch_wide<false, 128>(d, p.a, u.a_ld, p.n_entries, p.group2, st)
+           : launch_wide<false, 64>(d, p.a, u.a_ld, p.n_entries, p.group2, st);
   if (e != cudaSuccess) return e;
   for (int t0 = 0; t0 < p.T; t0 += 32768) {  // grid.y limit
     const int n = p.T - t0 < 32768 ? p.T - t0 : 32768;
