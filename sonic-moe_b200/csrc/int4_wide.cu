@@ -436,8 +436,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 // entries of each token.  The order of an expert's entries is that of shared-memory atomics: it decides
 // which column of a product an entry takes, and no column's value depends on that.  (For more entries,
 // the tiled kernels of router.cu.)
-constexpr int kPlanMaxEntries = 32768, kPlanMaxExperts = 1024;
+constexpr int kPlanMaxEntries = 16384, kPlanMaxExperts = 1024;
 
+template <int kPer>  // entries of a thread
 __global__ void __launch_bounds__(1024)
     wide_plan_kernel(const int32_t* __restrict__ experts, const int32_t* __restrict__ tokens, int n, int T, int K, int E,
                      int32_t* __restrict__ freq, int32_t* __restrict__ off, int32_t* __restrict__ s_rev,
@@ -445,16 +446,20 @@ __global__ void __launch_bounds__(1024)
   __shared__ int32_t s_cnt[kPlanMaxExperts], s_sum[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
+  int e[kPer], rank[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) e[i] = tid + 1024 * i < n ? experts[tid + 1024 * i] : -1;
   s_cnt[tid] = 0;
   if (clear_err && tid == 0) *err = 0;
   __syncthreads();
-#pragma unroll 4
-  for (int f = tid; f < n; f += 1024) {
-    const int e = experts[f];
-    if (e >= 0 && e < E)
-      s_rev[f] = atomicAdd(&s_cnt[e], 1);
-    else
-      atomicCAS(err, 0, kErrBadExpert);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (e[i] >= 0 && e[i] < E) {
+      rank[i] = atomicAdd(&s_cnt[e[i]], 1);
+    } else {
+      if (tid + 1024 * i < n) atomicCAS(err, 0, kErrBadExpert);
+      e[i] = -1;
+    }
   }
   __syncthreads();
   const int count = s_cnt[tid];  // zero beyond E
@@ -474,11 +479,11 @@ __global__ void __launch_bounds__(1024)
     off[tid] = base;
   }
   __syncthreads();
-#pragma unroll 4
-  for (int f = tid; f < n; f += 1024) {
-    const int e = experts[f];
-    if (e >= 0 && e < E) {
-      const int pos = s_cnt[e] + s_rev[f];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int f = tid + 1024 * i;
+    if (e[i] >= 0) {
+      const int pos = s_cnt[e[i]] + rank[i];
       s_rev[f] = pos;
       x_gather[pos] = tokens ? tokens[f] : f / K;
     }
@@ -541,30 +546,49 @@ __global__ void __launch_bounds__(256)
 }
 
 // out[t] = sum over t's entries f, [t K, (t + 1) K) or [tok_off[t], tok_off[t + 1]), of scores[f] times
-// the row y[s_rev[f]], in entry order, rounded once.  Entries whose expert was rejected have no row.
+// the row y[s_rev[f]], in entry order, rounded once.  Entries whose expert was rejected have no row.  A
+// warp's lanes look up 8 entries at a time, then all their rows are on the way together.
 __global__ void __launch_bounds__(256)
     wide_combine_kernel(const float* __restrict__ y, int T, int H, int K, const int32_t* __restrict__ tok_off,
                         const int32_t* __restrict__ experts, const float* __restrict__ scores,
                         const int32_t* __restrict__ s_rev, int E, __nv_bfloat16* __restrict__ out) {
   pdl_wait();
-  const int t = blockIdx.y;
+  const int t = blockIdx.y, lane = threadIdx.x & 31;
   const int c = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-  if (c >= H) return;
   const int f0 = tok_off ? tok_off[t] : t * K, f1 = tok_off ? tok_off[t + 1] : (t + 1) * K;
+  const float* col = y + (c < H ? c : 0);
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int f = f0; f < f1; ++f) {
-    const int e = experts[f];
-    if (e < 0 || e >= E) continue;
-    const float4 v = *reinterpret_cast<const float4*>(y + static_cast<size_t>(s_rev[f]) * H + c);
-    const float w = scores[f];
-    s.x = fmaf(w, v.x, s.x);
-    s.y = fmaf(w, v.y, s.y);
-    s.z = fmaf(w, v.z, s.z);
-    s.w = fmaf(w, v.w, s.w);
+  for (int f = f0; f < f1; f += 8) {
+    int row = -1;
+    float w = 0.0f;
+    if (lane < 8 && f + lane < f1) {
+      const int e = experts[f + lane];
+      if (e >= 0 && e < E) row = s_rev[f + lane];
+      w = scores[f + lane];
+    }
+    float4 v[8];
+    float ws[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = __shfl_sync(0xffffffffu, row, k);
+      ws[k] = __shfl_sync(0xffffffffu, w, k);
+      v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r >= 0)
+        v[k] = __ldcs(reinterpret_cast<const float4*>(col + static_cast<size_t>(r) * H));
+      else
+        ws[k] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s.x = fmaf(ws[k], v[k].x, s.x);
+      s.y = fmaf(ws[k], v[k].y, s.y);
+      s.z = fmaf(ws[k], v[k].z, s.z);
+      s.w = fmaf(ws[k], v[k].w, s.w);
+    }
   }
-  *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + c) =
-      make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
+  if (c < H)
+    *reinterpret_cast<uint2*>(out + static_cast<size_t>(t) * H + c) =
+        make_uint2(pack_bf16x2_rn(s.x, s.y), pack_bf16x2_rn(s.z, s.w));
 }
 
 template <bool kUp, int kN, int GPB>
@@ -600,8 +624,8 @@ bool int4_plan_fits(int n_entries, int E) { return n_entries <= kPlanMaxEntries 
 cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int n, int T, int K, int E, int32_t* freq,
                              int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
                              bool clear_err, cudaStream_t st) {
-  wide_plan_kernel<<<1, 1024, 0, st>>>(experts, tokens, n, T, K, E, freq, off, s_rev, x_gather, tok_off, err,
-                                          clear_err);
+  auto kern = n <= 1024 ? wide_plan_kernel<1> : n <= 4096 ? wide_plan_kernel<4> : wide_plan_kernel<16>;
+  kern<<<1, 1024, 0, st>>>(experts, tokens, n, T, K, E, freq, off, s_rev, x_gather, tok_off, err, clear_err);
   return cudaGetLastError();
 }
 
