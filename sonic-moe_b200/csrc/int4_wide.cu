@@ -302,9 +302,6 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
-      if (quarter == 0 &&
-          !warp_wait(&full_b[step % kStages], (step / kStages) & 1, p.err, kErrTimeoutProducer))
-        break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&full_a[group]);
     }
@@ -398,7 +395,8 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       const uint32_t d = tmem + (2 * buf + half) * kN;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
         const int s = step % kStages, g = 2 * (step & 1) + half;
-        if (!warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) {
+        if (!warp_wait(&full_b[s], (step / kStages) & 1, p.err, kErrTimeoutMma) ||
+            !warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
