@@ -10,8 +10,9 @@
 // nearly balanced routing would otherwise bring.)
 //
 // switch_loss_kernel        one pass over the logits: softmax of each row in registers, its columns
-//                           summed per thread, then over the CTA; counts of the top-k indices beside it.
-// switch_loss_finish_kernel adds the CTAs' sums in a fixed order (no floating-point atomics: the loss
+//                           summed per thread, over the CTA and over a cluster of 8 CTAs; counts of the
+//                           top-k indices beside it.
+// switch_loss_finish_kernel adds the clusters' sums in a fixed order (no floating-point atomics: the loss
 //                           is the same bits every time) and forms the loss and c.
 // switch_loss_bwd_kernel    reads the logits once more, recomputes the softmax, writes the gradient.
 #include "common.cuh"
@@ -22,6 +23,8 @@ namespace smb {
 namespace {
 
 constexpr int kSlThreads = 256;
+constexpr int kSlCluster = 8;       // CTAs of the forward that add their sums before they write them
+constexpr int kSlMaxParts = 4 * 18;  // clusters at most (148 SMs hold 18)
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -37,26 +40,32 @@ __device__ __forceinline__ void from_f32(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __half* p) { *p = __float2half_rn(v); }
 
-// 8 consecutive values; vec: how many of them one aligned access may cover (8, 4 or 1).
+// 8 consecutive values as loaded; vec: how many of them one aligned access may cover (8, 4 or 1).
 template <typename InT>
-__device__ __forceinline__ void load8(const InT* __restrict__ src, int vec, int n, float* v) {
-  alignas(16) InT raw[8];
+struct Raw8 {
+  alignas(16) InT v[8];
+};
+template <typename InT>
+__device__ __forceinline__ void load8(const InT* __restrict__ src, int vec, int n, Raw8<InT>& raw) {
   if (vec >= 4 && n >= 8) {
     if constexpr (sizeof(InT) == 4) {
-      *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(src));
-      *reinterpret_cast<uint4*>(raw + 4) = __ldg(reinterpret_cast<const uint4*>(src + 4));
+      *reinterpret_cast<uint4*>(raw.v) = __ldg(reinterpret_cast<const uint4*>(src));
+      *reinterpret_cast<uint4*>(raw.v + 4) = __ldg(reinterpret_cast<const uint4*>(src + 4));
     } else if (vec == 8) {
-      *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(src));
+      *reinterpret_cast<uint4*>(raw.v) = __ldg(reinterpret_cast<const uint4*>(src));
     } else {
-      *reinterpret_cast<uint2*>(raw) = __ldg(reinterpret_cast<const uint2*>(src));
-      *reinterpret_cast<uint2*>(raw + 4) = __ldg(reinterpret_cast<const uint2*>(src + 4));
+      *reinterpret_cast<uint2*>(raw.v) = __ldg(reinterpret_cast<const uint2*>(src));
+      *reinterpret_cast<uint2*>(raw.v + 4) = __ldg(reinterpret_cast<const uint2*>(src + 4));
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32(raw[j]);
     return;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(src[j]) : -__int_as_float(0x7f800000);
+  for (int j = 0; j < 8; ++j) {
+    if (j < n)
+      raw.v[j] = src[j];
+    else
+      from_f32(-__int_as_float(0x7f800000), &raw.v[j]);
+  }
 }
 
 template <typename InT>
@@ -120,11 +129,37 @@ __device__ __forceinline__ float softmax_row(float (&v)[8 * C], float* s_red) {
   return 1.0f / row_reduce<L, false>(s, s_red);
 }
 
-// Lane layout: group lane l holds columns 8 l + 8 L c + (0..7), c < C; E <= 8 L C.
+// Lane layout: group lane l holds columns 8 l + 8 L c + (0..7), c < C; E <= 8 L C.  A row that does not
+// count is not read (zeros stand in).
 template <typename InT, int L, int C>
-__device__ __forceinline__ void load_row(const InT* __restrict__ row, int E, int vec, int gl, float (&v)[8 * C]) {
+__device__ __forceinline__ void load_row(const InT* __restrict__ row, bool on, int E, int vec, int gl,
+                                         Raw8<InT> (&raw)[C]) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) load8<InT>(row + 8 * gl + 8 * L * c, vec, E - 8 * gl - 8 * L * c, v + 8 * c);
+  for (int c = 0; c < C; ++c) {
+    if (on) {
+      load8<InT>(row + 8 * gl + 8 * L * c, vec, E - 8 * gl - 8 * L * c, raw[c]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) from_f32(0.0f, &raw[c].v[j]);
+    }
+  }
+}
+template <typename InT, int C>
+__device__ __forceinline__ void row_f32(const Raw8<InT> (&raw)[C], float (&v)[8 * C]) {
+#pragma unroll
+  for (int i = 0; i < 8 * C; ++i) v[i] = to_f32(raw[i / 8].v[i % 8]);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The 32-bit word at this CTA's shared address `p`, in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t ld_cluster(const void* p, int rank) {
+  uint32_t a, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
 }
 
 // Loss and gradient coefficients from the column sums: thread i of the CTA calls with every e it owns.
@@ -182,30 +217,34 @@ __global__ void __launch_bounds__(kSlThreads)
                        const int32_t* __restrict__ idx, int K, const int32_t* __restrict__ freq_in,
                        float* __restrict__ part_p, int32_t* __restrict__ part_f, float* __restrict__ loss,
                        float* __restrict__ coef, int32_t* __restrict__ freq_out, int* __restrict__ err) {
-  constexpr int kGroups = kSlThreads / L;               // rows in flight per CTA
+  constexpr int kGroups = kSlThreads / L;               // rows of a CTA's step
   constexpr int kCopies = L < 32 ? kSlThreads / 32 : kGroups;
   extern __shared__ float s_dyn[];
   __shared__ float s_red[8];
   float* s_p = s_dyn;
   int32_t* s_f = reinterpret_cast<int32_t*>(s_dyn + static_cast<size_t>(kCopies) * E);
   const int gl = threadIdx.x % L, grp = threadIdx.x / L;
+  pdl_launch();
   if (idx)
     for (int e = threadIdx.x; e < E; e += kSlThreads) s_f[e] = 0;
   float acc[8 * C];
 #pragma unroll
   for (int i = 0; i < 8 * C; ++i) acc[i] = 0.0f;
-  // every group takes the same number of rows, so that the shuffles and barriers below are uniform
-  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T;
-       r0 += static_cast<long long>(gridDim.x) * kGroups) {
-    const long long r = r0 + grp;
-    const bool on = r < T && (!mask || mask[r]);
+  // every group takes the same number of rows, so that the shuffles and barriers below are uniform; the
+  // next row is under way while one is reduced
+  const long long stride = static_cast<long long>(gridDim.x) * kGroups;
+  auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + grp;
+  Raw8<InT> next[C];
+  bool on_next = counts(r);
+  load_row<InT, L, C>(logits + r * E, on_next, E, vec, gl, next);
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += stride) {
     float v[8 * C];
-    if (on) {
-      load_row<InT, L, C>(logits + r * E, E, vec, gl, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8 * C; ++i) v[i] = 0.0f;
-    }
+    row_f32<InT, C>(next, v);
+    const bool on = on_next;
+    r += stride;
+    on_next = counts(r);
+    load_row<InT, L, C>(logits + r * E, on_next, E, vec, gl, next);
     const float inv = softmax_row<L, C>(v, s_red);
     if (on) {
 #pragma unroll
@@ -245,21 +284,33 @@ __global__ void __launch_bounds__(kSlThreads)
   for (int e = threadIdx.x; e < E; e += kSlThreads) {
     float p = s_p[e];
     for (int k = 1; k < kCopies; ++k) p += s_p[static_cast<size_t>(k) * E + e];
-    if (gridDim.x == 1) {
-      s_p[e] = p;
-      if (!idx) s_f[e] = freq_in[e];
-    } else {
-      part_p[static_cast<size_t>(blockIdx.x) * E + e] = p;
-      if (idx) part_f[static_cast<size_t>(blockIdx.x) * E + e] = s_f[e];
-    }
+    s_p[e] = p;
+    if (gridDim.x == 1 && !idx) s_f[e] = freq_in[e];
   }
   if (gridDim.x == 1) {
     __syncthreads();
     finish(s_p, s_f, E, loss, coef, freq_out);
+    return;
   }
+  // the cluster's CTAs each add an eighth of the columns over all 8
+  cluster_sync();
+  const int rank = blockIdx.x % kSlCluster;
+  const size_t part = static_cast<size_t>(blockIdx.x / kSlCluster) * E;
+  for (int e = rank * kSlThreads + threadIdx.x; e < E; e += kSlCluster * kSlThreads) {
+    float p = 0.0f;
+    int f = 0;
+#pragma unroll
+    for (int k = 0; k < kSlCluster; ++k) {
+      p += __uint_as_float(ld_cluster(&s_p[e], k));
+      if (idx) f += static_cast<int>(ld_cluster(&s_f[e], k));
+    }
+    part_p[part + e] = p;
+    if (idx) part_f[part + e] = f;
+  }
+  cluster_sync();  // nobody's shared memory goes away while it is read
 }
 
-// The CTAs' sums, `slices` groups of threads each adding every slices-th part, then the groups in order.
+// The clusters' sums, `slices` groups of threads each adding every slices-th part, then the groups in order.
 constexpr int kFinThreads = 1024;
 constexpr int kFinSlots = 4096;  // slices * E <= kFinSlots
 
@@ -269,6 +320,7 @@ __global__ void __launch_bounds__(kFinThreads)
                               float* __restrict__ coef, int32_t* __restrict__ freq_out) {
   __shared__ float s_p[kFinSlots];
   __shared__ int32_t s_f[kFinSlots];
+  pdl_wait();
   for (int i = threadIdx.x; i < slices * E; i += kFinThreads) {
     const int sl = i / E, e = i - sl * E;
     float p = 0.0f;
@@ -313,17 +365,20 @@ __global__ void __launch_bounds__(kSlThreads)
       const int e = 8 * gl + 8 * L * k + j;
       c[8 * k + j] = e < E ? coef[e] : 0.0f;
     }
-  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T;
-       r0 += static_cast<long long>(gridDim.x) * kGroups) {
-    const long long r = r0 + grp;
-    const bool on = r < T && (!mask || mask[r]);
+  const long long stride = static_cast<long long>(gridDim.x) * kGroups;
+  auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
+  long long r_next = static_cast<long long>(blockIdx.x) * kGroups + grp;
+  Raw8<InT> next[C];
+  bool on_next = counts(r_next);
+  load_row<InT, L, C>(logits + r_next * E, on_next, E, vec, gl, next);
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += stride) {
     float v[8 * C];
-    if (on) {
-      load_row<InT, L, C>(logits + r * E, E, vec, gl, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8 * C; ++i) v[i] = 0.0f;
-    }
+    row_f32<InT, C>(next, v);
+    const long long r = r_next;
+    const bool on = on_next;
+    r_next += stride;
+    on_next = counts(r_next);
+    load_row<InT, L, C>(logits + r_next * E, on_next, E, vec, gl, next);
     const float inv = softmax_row<L, C>(v, s_red);
     float dot = 0.0f;
 #pragma unroll
@@ -378,16 +433,33 @@ cudaError_t launch_lc(const SlArgs& a, bool bwd, cudaStream_t st) {
   }
   constexpr int kCopies = L < 32 ? kSlThreads / 32 : kSlThreads / L;
   const int smem = (kCopies + 1) * a.E * 4;
-  switch_loss_kernel<InT, L, C><<<a.grid, kSlThreads, smem, st>>>(
-      x, a.T, a.E, vec_of(a.logits, a.E, sizeof(InT)), a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss,
-      a.coef, a.freq_out, a.err);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.grid == 1) return e;
+  auto kern = switch_loss_kernel<InT, L, C>;
+  const int vec = vec_of(a.logits, a.E, sizeof(InT));
+  cudaError_t e;
+  if (a.grid == 1) {
+    kern<<<1, kSlThreads, smem, st>>>(x, a.T, a.E, vec, a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss, a.coef,
+                                      a.freq_out, a.err);
+    return cudaGetLastError();
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.grid * kSlCluster);
+  cfg.blockDim = dim3(kSlThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = kSlCluster;
+  at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, x, a.T, a.E, vec, a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss, a.coef,
+                         a.freq_out, a.err);
+  if (e != cudaSuccess) return e;
   const int slices = a.E >= kFinThreads ? 1 : kFinThreads / a.E;
-  switch_loss_finish_kernel<<<1, kFinThreads, 0, st>>>(a.part_p, a.idx ? a.part_f : nullptr, a.grid, a.E,
-                                                       slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef,
-                                                       a.freq_out);
-  return cudaGetLastError();
+  return launch_dependent(switch_loss_finish_kernel, dim3(1), kFinThreads, 0, 1, st, a.part_p,
+                          a.idx ? a.part_f : nullptr, a.grid, a.E, slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef,
+                          a.freq_out);
 }
 
 // Lanes per row: as many as hold the row at 8 values each, up to a warp; wider rows take 16 or 32
@@ -418,10 +490,11 @@ cudaError_t launch(const SlArgs& a, int dtype, bool bwd, cudaStream_t st) {
 
 }  // namespace
 
+// Rows of the partial sums: one CTA does it all where that takes at most 8 steps, else clusters of 8.
 int switch_loss_parts(int T, int E) {
-  const int rows = 8 * (kSlThreads / lanes_of(E));  // at least 8 steps a CTA
-  const int want = ceil_div(T, rows);
-  return want < 1 ? 1 : want > 2 * 148 ? 2 * 148 : want;
+  const int ctas = ceil_div(T, 8 * (kSlThreads / lanes_of(E)));
+  const int want = ceil_div(ctas, kSlCluster);
+  return ctas <= 1 ? 1 : want < 2 ? 2 : want > kSlMaxParts ? kSlMaxParts : want;
 }
 
 cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,

@@ -325,4 +325,29 @@ __device__ __forceinline__ void store_tile_transposed_128(const uint8_t* tile, u
     *reinterpret_cast<uint4*>(d + static_cast<size_t>(b) * ld) = make_uint4(r[b][0], r[b][1], r[b][2], r[b][3]);
 }
 
+// --------------------------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel may start while its predecessor drains, and waits for its results.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t st,
+                             A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 }  // namespace smb

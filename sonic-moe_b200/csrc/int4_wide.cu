@@ -19,16 +19,22 @@
 //   warps 16-19  epilogue: rows 32 (w % 4) .. of the accumulators of the two halves
 //   warp 20      TMA producer of x
 //   warps 21-22  MMA issuers, one for each half of the rows (21 allocates tensor memory)
-// An issuer's waits and commits cost it some hundred cycles a step whatever they guard, as long as its 8
-// MMAs of 64 tokens take (32 cycles each).  So a step has 128 columns, the halves have an issuer each,
-// whose work the tensor core interleaves, and an issuer waits once and commits once a step: that x has
-// landed is waited for by the dequantising warps, before they announce their part.  An item has 256 rows
-// because x, which every row tile reads from L2, otherwise costs an SM twice the bytes of the weights
-// (64 tokens: 16 KB a step against 8 KB).
+// An issuer's waits and its commit cost it some hundred cycles a step whatever they guard, as long as its
+// 8 MMAs of 64 tokens take (32 cycles each, measured).  So a step has 128 columns and the halves have an
+// issuer each, whose work the tensor core interleaves.  An item has 256 rows because x, which every row
+// tile reads from L2, otherwise costs an SM twice the bytes of the weights (64 tokens: 16 KB a step
+// against 8 KB).
 // Work items (expert, 256 rows, up to kN of its tokens), rows fastest, static round robin; the items of
 // an expert's token chunks follow each other, so their second reading of the weights is from L2.  kN is
-// 64 with double-buffered accumulators (the epilogue overlaps the next item), or 128 with single ones,
-// which halves the dequantising per token.
+// 64 or 128; 128 halves the dequantising per token, 64 leaves room for a third stage of weights in tensor
+// memory.
+// What bounds it (512 tokens, 64 experts of 4096 x 1024): the dequantising warps.  Per SM a step of 256
+// rows takes about 1000 cycles, against 790 for its bytes at the HBM rate and 512 for its MMAs; 7 of the 11
+// instructions for 8 weights are integer ones, which an SM issues at half rate (448 cycles of the step).
+// Fetching the codes by bulk copies from a warp of their own instead of per-lane copies, which takes a
+// tenth of the instructions away but adds a barrier wait to every step, measured 117 us against 104 (up
+// projection); double-buffered accumulators instead of the third stage of weights 239 against 228 us
+// (64 tokens, 128 experts).
 // Every wait is bounded; after a time-out the kernel records an error, drains and returns.
 #include "int4.cuh"
 
@@ -37,17 +43,14 @@ namespace smb {
 namespace {
 
 constexpr int kWdDeqWarps = 16;
-constexpr int kWdGroups = kWdDeqWarps / 4;  // 4 warps store the 128 rows of half an item
 constexpr int kWdThreads = 32 * (kWdDeqWarps + 7);
-constexpr uint32_t kWdTmemA = 256;  // accumulators below, A stages of 64 columns from here
-
 template <int kN>  // tokens of an item at most
 struct WdShape {
-  static constexpr int kBufs = 128 / kN;  // accumulator buffers of two halves of kN columns
+  static constexpr uint32_t kTmemA = 2 * kN;  // accumulators of the two halves below, stages of A from here
+  static constexpr int kAStages = (512 - 2 * kN) / 128;
   static constexpr int kBHalf = kN * 128;  // 64 columns of x
   static constexpr int kBStage = 2 * kBHalf;
   static constexpr int kStages = 98304 / kBStage;  // 128-column steps of x in shared memory
-  static_assert(kBufs * 2 * kN == 256, "accumulators fill the columns below kWdTmemA");
 };
 
 template <int GPB>
@@ -119,11 +122,12 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     wide_kernel(const __grid_constant__ CUtensorMap tmap_x16, const __grid_constant__ CUtensorMap tmap_x64,
                 const WdArgs p) {
   using Shape = WdShape<kN>;
-  constexpr int kStages = Shape::kStages, kBufs = Shape::kBufs;
+  constexpr int kStages = Shape::kStages;
   extern __shared__ uint8_t smem_raw[];
-  // step n, half h: full_a[2 (n % 2) + h] both operands are there, done[h][n % kStages] the MMAs have read
-  // them; full_b[n % kStages] x is there
-  __shared__ uint64_t full_a[kWdGroups], full_b[kStages], done[2][kStages], tfull[kBufs], tempty[kBufs], drain[2];
+  // step n, half h: full_a[h][n % kA] the weights are there, full_b[n % kStages] x is, done[h][n % kStages] the
+  // MMAs have read both
+  constexpr int kA = Shape::kAStages;
+  __shared__ uint64_t full_a[2][kA], full_b[kStages], done[2][kStages], tfull, tempty, drain[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int32_t s_warp[kWdThreads / 32];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -133,16 +137,15 @@ __global__ void __launch_bounds__(kWdThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int g = 0; g < kWdGroups; ++g) mbar_init(&full_a[g], 4);
+    for (int s = 0; s < kA; ++s)
+      for (int h = 0; h < 2; ++h) mbar_init(&full_a[h][s], 4);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_b[s], 1);
       mbar_init(&done[0][s], 1);
       mbar_init(&done[1][s], 1);
     }
-    for (int i = 0; i < kBufs; ++i) {
-      mbar_init(&tfull[i], 2);
-      mbar_init(&tempty[i], 4);
-    }
+    mbar_init(&tfull, 2);
+    mbar_init(&tempty, 4);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     fence_mbar_init();
@@ -203,8 +206,9 @@ __global__ void __launch_bounds__(kWdThreads, 1)
 
   if (warp < kWdDeqWarps) {
     // ---------------------------------------------------------------- dequantise
-    // Steps are numbered through all items of the CTA; a group takes every other one, and one half of the
-    // rows, into the stage of tensor memory that is its own.
+    // Steps are numbered through all items of the CTA; a group takes every other one.  A parity wait may
+    // not fall two phases behind its barrier; here it cannot, since the wait for a step's MMAs implies that
+    // every earlier use of the barriers is over.
     constexpr int kStage = WdRing<GPB>::kStage, kDepth = WdRing<GPB>::kDepth;
     const Int4Magic magic;
     const int quarter = warp & 3, group = warp >> 2, half = group & 1, odd = group >> 1, g = lane >> 2;
@@ -288,14 +292,14 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           }
         }
         if (j == 0) {  // the first tile is ready while the MMAs still read the stage
-          if (step >= 2 && !warp_wait(&done[half][(step - 2) % kStages], ((step - 2) / kStages) & 1, p.err,
-                                      kErrTimeoutProducer)) {
+          if (step >= kA && !warp_wait(&done[half][(step - kA) % kStages], ((step - kA) / kStages) & 1, p.err,
+                                       kErrTimeoutProducer)) {
             ok = false;
             break;
           }
           tc_fence_after();
         }
-        const uint32_t dst = tmem + kWdTmemA + 64 * group + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16);
+        const uint32_t dst = tmem + Shape::kTmemA + 128 * (step % kA) + 64 * half + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16);
         tmem_st_16x32(dst, r[0]);
         tmem_st_16x32(dst + 32, r[1]);
       }
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_a[group]);
+      if (lane == 0) mbar_arrive(&full_a[half][step % kA]);
     }
     cp_async_wait<0>();
   } else if (warp < kWdDeqWarps + 4) {
@@ -312,14 +316,13 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     int li = 0;
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++li) {
       const WdItem it = item_of(i);
-      const int buf = li % kBufs;
-      if (!warp_wait(&tfull[buf], (li / kBufs) & 1, p.err, kErrTimeoutEpilogue)) break;
+      if (!warp_wait(&tfull, li & 1, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const int pieces = (it.n + 31) / 32;
       for (int piece = 0; piece < 2 * pieces; ++piece) {  // half of the rows, 32 tokens
         const int half = piece >= pieces, c0 = 32 * (piece - half * pieces);
         uint32_t v[32];
-        tmem_ld32(tmem + (2 * buf + half) * kN + c0 + (static_cast<uint32_t>(32 * quarter) << 16), v);
+        tmem_ld32(tmem + half * kN + c0 + (static_cast<uint32_t>(32 * quarter) << 16), v);
         tmem_ld_wait();
         const int n = min(32, it.n - c0);
         if (kUp) {
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
+      if (lane == 0) mbar_arrive(&tempty);
     }
   } else if (warp == kWdDeqWarps + 4) {
     // ---------------------------------------------------------------- TMA producer of x
@@ -389,20 +392,19 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
       const int n = __shfl_sync(0xffffffffu, item_of(i).n, 0);
       const uint32_t idesc = wd_idesc((n + 15) & ~15);
-      const int buf = li % kBufs;
-      if (!warp_wait(&tempty[buf], ((li / kBufs) & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      if (!warp_wait(&tempty, (li & 1) ^ 1, p.err, kErrTimeoutMma)) break;
       tc_fence_after();
-      const uint32_t d = tmem + (2 * buf + half) * kN;
+      const uint32_t d = tmem + half * kN;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
-        const int s = step % kStages, g = 2 * (step & 1) + half;
+        const int s = step % kStages, g = step % kA;
         if (!warp_wait(&full_b[s], (step / kStages) & 1, p.err, kErrTimeoutMma) ||
-            !warp_wait(&full_a[g], (step >> 1) & 1, p.err, kErrTimeoutMma)) {
+            !warp_wait(&full_a[half][g], (step / kA) & 1, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint64_t bd = sdesc_sw128(smem_u32(smem + s * Shape::kBStage));
-        const uint32_t a = tmem + kWdTmemA + 64 * g;
+        const uint32_t a = tmem + Shape::kTmemA + 128 * g + 64 * half;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // 16 columns per MMA: 8 columns of A, 32 bytes of B
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         }
         __syncwarp();
       }
-      if (ok && elect_one()) tc_commit(&tfull[buf]);
+      if (ok && elect_one()) tc_commit(&tfull);
       __syncwarp();
     }
     if (elect_one()) {

@@ -79,7 +79,7 @@ cudaError_t launch_tq_pack(const void* src, int C, int src_padded, const int32_t
 cudaError_t launch_router_bwd(const void* logits, const float* scores, const int32_t* idx, const float* ds, int T,
                               int E, int K, int sot, int renorm, float* dlogits, cudaStream_t st);
 
-// router balance loss (csrc/balance.cu); parts = CTAs of the forward = rows of part_p / part_f [parts, E]
+// router balance loss (csrc/balance.cu); parts = rows of the partial sums part_p / part_f [parts, E]
 int switch_loss_parts(int T, int E);
 cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,
                                int K, const int32_t* freq_in, float* part_p, int32_t* part_f, float* loss,
