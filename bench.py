@@ -541,7 +541,7 @@ def run_side_workload(args):
     import torch
 
     from sonicmoe import ops
-    from sonicmoe.functional import moe_general_routing_inputs, moe_TC_softmax_topk_layer
+    from sonicmoe.functional import moe_general_routing_inputs, moe_TC_softmax_topk_layer, prepare_int4_weights
 
     T, H, I, E, K, desc = SIDE_WORKLOADS[args.workload]
     dev = torch.device("cuda", 0)
@@ -572,9 +572,13 @@ def run_side_workload(args):
         sc = scores.reshape(-1).contiguous()
         tok = torch.arange(T, dtype=torch.int32, device=dev).repeat_interleave(K)
         ex = idx.reshape(-1).to(torch.int32).contiguous()
+        w1e, w2e = w1v, w2v
+        if args.expert_bits == 4:
+            w1e, w2e = prepare_int4_weights(w1v), prepare_int4_weights(w2v)
+            desc += ", 4-bit expert weights with a scale per 128 columns"
 
         def forward():
-            moe_general_routing_inputs(x, sc, tok, ex, w1v, None, w2v, None, E, None, is_inference_mode_enabled=True)
+            moe_general_routing_inputs(x, sc, tok, ex, w1e, None, w2e, None, E, None, is_inference_mode_enabled=True)
     stream = torch.cuda.Stream(device=dev)
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
@@ -604,8 +608,10 @@ def run_side_workload(args):
         line["roofline"] = {"bound": "tensor", "achieved": tf, "peak": 2 * peaks["bf16_tflops"], "unit": "TFLOP/s",
                             "frac": tf / (2 * peaks["bf16_tflops"]), "peak_source": src}
     else:
-        # e4m3 weights of the experts the batch touches, plus their 128x128 scale bytes
-        wbytes = active * (3 * H * I + 3 * H * I // (128 * 128))
+        # weights of the experts the batch touches: e4m3 plus a scale byte per 128 x 128 block, or 4-bit codes
+        # plus a bf16 scale per 128 columns of a row
+        wbytes = active * (3 * H * I // 2 + 2 * (3 * H * I // 128) if args.expert_bits == 4 else
+                           3 * H * I + 3 * H * I // (128 * 128))
         gbs = wbytes / (ms / 1e3) / 1e9
         line["active_experts"] = active
         line["roofline"] = {"bound": "hbm", "achieved": gbs, "peak": peaks["hbm_gbs"], "unit": "GB/s",
@@ -632,6 +638,8 @@ def main():
     ap.add_argument("--workload", choices=["c2"] + sorted(SIDE_WORKLOADS), default="c2",
                     help="c2 = the headline configuration (default, the contract line); the others time the "
                          "benchmark's remaining configurations (c4 also expert parallel with --gpus N > 1)")
+    ap.add_argument("--expert-bits", type=int, choices=[4, 8], default=8,
+                    help="decoding workloads (c5_64, c5_512): 8 = the FP8 engine, 4 = 4-bit expert weights")
     ap.add_argument("--train", action="store_true",
                     help="time one GPU's training step (forward + FP8 backward) of config 2 instead of the forward")
     ap.add_argument("--profile", action="store_true",

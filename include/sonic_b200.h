@@ -495,7 +495,7 @@ int sm_switch_loss_bwd(const void* router_logits, int dtype, int T, int E, const
  * columns of a row: the smallest number of 5 significant bits (at least 2^-126) that is >= amax / 7;
  * code = w / scale to nearest, ties to even.  Every code times its scale is exactly a bf16 number.
  * wq [sm_int4_weight_bytes] and scales [sm_int4_scale_count] bf16 are in this library's own order
- * (16-byte aligned).  A group holding an infinity or NaN gets a NaN scale.
+ * (16-byte aligned).  |w| < 2^124; a group holding an infinity or NaN gets a NaN scale.
  */
 size_t sm_int4_weight_bytes(int E, int N, int K);
 size_t sm_int4_scale_count(int E, int N, int K, int group);

@@ -147,20 +147,24 @@ constexpr int kMvThreads = 32 * kMvWarps;
 
 // ---------------------------------------------------------------------------------------------
 // Few tokens.  Two launches: the up projection and the down projection with the sum over a token's
-// experts.  Both read each weight of an active expert once and are bound by those bytes, so what counts
-// is how many loads are in flight:
+// experts.  Both read each weight of an active expert once:
 //   - every warp streams row tiles of its own (MT x 16 rows) through a ring of kDepth column blocks in
 //     shared memory, filled by 16-byte asynchronous copies ahead of the products, across the end of one
 //     tile and the start of the next; a lane reads back only what it copied itself, so the ring needs no
 //     barrier;
 //   - there is no routing pass: every CTA makes the list of active experts and their entries itself from
-//     the (few) expert ids while its first loads could not be issued anyway;
+//     the (few) expert ids;
 //   - the down kernel starts while the up kernel drains (programmatic dependent launch) and has its first
-//     weights in registers before it waits for the intermediate.
+//     weights on the way before it waits for the intermediate.
 // The m16n8k16 tensor core product takes 8 tokens as its 8 columns; with one token 7/8 of its work is
 // thrown away, but it still keeps up with the memory, which the plain FMA units would not beyond 2 tokens.
+// What bounds it: integer instructions, which an SM issues at half rate.  Turning 2048 codes into bf16 takes
+// a warp 56 of them (28 cycles of an SM) and some 25 for the ring, against 44 cycles that their bytes take
+// at the HBM rate; with the latencies in between the layer streams at 3.3 TB/s (8 tokens, 4096 x 1024, 128
+// experts: 107 us; one token 28.6 us).  Registers instead of the shared-memory ring, a block of x without the
+// read-ahead, and 1 or 4 row tiles a warp all measured slower.
 
-constexpr int kSmMaxEntries = 1024;
+constexpr int kSmMaxEntries = 256;  // their down results are kept in shared memory (128 bytes an entry)
 
 // Active experts (slots, ascending) of the entries and their flat entries, slot s owning
 // list[beg[s]] .. list[beg[s + 1]).  The order inside a slot does not matter: an entry's values do not

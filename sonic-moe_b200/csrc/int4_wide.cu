@@ -56,7 +56,8 @@ struct WdShape {
 template <int GPB>
 struct WdRing {
   static constexpr int kStage = 2 * (1024 + 128 * GPB);  // a step of 2 row tiles, GPB scale words a lane
-  static constexpr int kDepth = GPB == 4 ? 2 : 3;        // steps of codes in flight per dequantising warp
+  // steps of codes in flight per dequantising warp: what fits beside x and 4096 experts' prefix
+  static constexpr int kDepth = GPB == 1 ? 3 : 2;
   static constexpr int kBytes = kWdDeqWarps * kDepth * kStage;
 };
 
@@ -594,6 +595,8 @@ __global__ void __launch_bounds__(256)
 template <bool kUp, int kN, int GPB>
 cudaError_t launch_wide(const CUtensorMap& t16, const CUtensorMap& t64, const WdArgs& p, int grid, cudaStream_t st) {
   const int smem = 1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
+  static_assert(1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes + 4097 * 4 <= 232448 - 1024,
+                "shared memory budget");
   auto kern = wide_kernel<kUp, kN, GPB>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;

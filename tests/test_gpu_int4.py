@@ -94,6 +94,8 @@ LAYER = [
     (1000, 256, 256, 7, 3, 128, False, 1.2),
     (40, 64, 24, 1100, 4, 32, False, 0.0),  # more experts, more entries than the one-launch routing plan takes
     (5000, 64, 16, 9, 7, 64, True, 1.2),
+    (10, 64, 24, 4096, 2, 64, False, 0.0),  # the most experts, on both paths
+    (3, 64, 24, 4096, 8, 32, False, 0.0),
 ]
 
 
@@ -115,7 +117,7 @@ def test_layer_topk(ops, T, H, I, E, K, group, concat, skew):
 
 
 @pytest.mark.parametrize("T,H,I,E,n", [(1, 128, 64, 4, 1), (1, 256, 64, 3, 9), (5, 72, 40, 3, 4), (40, 512, 256, 8, 133),
-                                       (64, 256, 128, 70, 500), (200, 264, 136, 5, 700), (900, 128, 64, 6, 2500)])
+                                       (64, 256, 128, 70, 500), (8, 512, 256, 4, 256), (8, 512, 256, 4, 257), (200, 264, 136, 5, 700), (900, 128, 64, 6, 2500)])
 def test_layer_lists(ops, T, H, I, E, n):
     """Explicit lists: tokens without entries, tokens with many, the same expert twice for a token."""
     w1, w2, g = _weights(E, H, I, T + n)
