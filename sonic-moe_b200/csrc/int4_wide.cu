@@ -44,6 +44,7 @@ namespace {
 
 constexpr int kWdDeqWarps = 16;
 constexpr int kWdThreads = 32 * (kWdDeqWarps + 7);
+
 template <int kN>  // tokens of an item at most
 struct WdShape {
   static constexpr uint32_t kTmemA = 2 * kN;  // accumulators of the two halves below, stages of A from here
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     // every earlier use of the barriers is over.
     constexpr int kStage = WdRing<GPB>::kStage, kDepth = WdRing<GPB>::kDepth;
     const Int4Magic magic;
-    const int quarter = warp & 3, group = warp >> 2, half = group & 1, odd = group >> 1, g = lane >> 2;
+    const int quarter = warp & 3, half = (warp >> 2) & 1, odd = warp >> 3, g = lane >> 2;
     const uint32_t ring = smem_u32(rings) + warp * kDepth * kStage;
     int l_item = blockIdx.x, l_b = odd, l_stage = 0, u_stage = 0;
     const uint8_t* l_src[2] = {};
@@ -265,21 +266,24 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     const int my_items = (items - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) /
                          static_cast<int>(gridDim.x);
     const int total = my_items * p.k_blocks;  // steps of this CTA
+    const uint32_t lanes = tmem + Shape::kTmemA + 64 * half + (static_cast<uint32_t>(32 * quarter) << 16);
     bool ok = true;
     for (int step = odd; step < total; step += 2) {
+      const int sa = step % kA;  // stage of tensor memory
       fill();  // the stage freed by the step before
       cp_async_wait<kDepth - 1>();
       const uint32_t st = ring + u_stage * kStage;
       if (++u_stage == kDepth) u_stage = 0;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint32_t sw[GPB], r[2][16];
+        uint32_t sw[GPB];
 #pragma unroll
         for (int i = 0; i < GPB; ++i) sw[i] = lds32(st + 2048 + j * 128 * GPB + 4 * GPB * lane + 4 * i);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // 64 columns
           const uint4 q = lds128(st + 1024 * j + 512 * h + 16 * lane);
           const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+          uint32_t r[16];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {  // 32 columns
             const uint32_t s = sw[(2 * h + k) * GPB / 4];
@@ -287,28 +291,24 @@ __global__ void __launch_bounds__(kWdThreads, 1)
             const __nv_bfloat162 ml = int4_m24(sl), mh = int4_m24(sh);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              r[h][2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
-              r[h][2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
+              r[2 * (4 * k + c)] = int4_scaled(magic, w[2 * k], c, sl, ml);
+              r[2 * (4 * k + c) + 1] = int4_scaled(magic, w[2 * k + 1], c, sh, mh);
             }
           }
-        }
-        if (j == 0) {  // the first tile is ready while the MMAs still read the stage
-          if (step >= kA && !warp_wait(&done[half][(step - kA) % kStages], ((step - kA) / kStages) & 1, p.err,
-                                       kErrTimeoutProducer)) {
-            ok = false;
-            break;
+          if (ok && j == 0 && h == 0) {  // the MMAs of the stage's last step
+            if (step >= kA)
+              ok = warp_wait(&done[half][(step - kA) % kStages], ((step - kA) / kStages) & 1, p.err,
+                             kErrTimeoutProducer);
+            tc_fence_after();
           }
-          tc_fence_after();
+          if (ok) tmem_st_16x32(lanes + 128 * sa + (static_cast<uint32_t>(16 * j) << 16) + 32 * h, r);
         }
-        const uint32_t dst = tmem + Shape::kTmemA + 128 * (step % kA) + 64 * half + (static_cast<uint32_t>(32 * quarter + 16 * j) << 16);
-        tmem_st_16x32(dst, r[0]);
-        tmem_st_16x32(dst + 32, r[1]);
       }
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_a[half][step % kA]);
+      if (lane == 0) mbar_arrive(&full_a[half][sa]);
     }
     cp_async_wait<0>();
   } else if (warp < kWdDeqWarps + 4) {
