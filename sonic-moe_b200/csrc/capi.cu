@@ -769,10 +769,9 @@ Int4Ws carve_int4(Carve& c, int T, int n_entries, int H, int I, int E) {
   w.s_rev = c.take<int32_t>(n_entries);
   w.x_gather = c.take<int32_t>(n_entries);
   w.tok_off = c.take<int32_t>(static_cast<size_t>(T) + 1);
-  const bool small = int4_small(T, n_entries);
-  w.xs = c.take<uint16_t>(small ? 0 : static_cast<size_t>(n_entries) * int4_padded(H));
+  w.xs = c.take<uint16_t>(static_cast<size_t>(n_entries) * int4_padded(H));
   w.a = c.take<uint16_t>(static_cast<size_t>(n_entries) * int4_padded(I));
-  w.y = c.take<float>(small ? 0 : static_cast<size_t>(n_entries) * H);
+  w.y = c.take<float>(static_cast<size_t>(n_entries) * H);
   w.err = c.take<int32_t>(1);
   return w;
 }
@@ -919,7 +918,7 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   p.y = w.y;
   p.out = out;
   p.err = err;
-  if (int4_small(T, n_entries)) return cuda_status(launch_int4_small(p, st), "moe_int4_forward");
+  if (int4_small(p)) return cuda_status(launch_int4_small(p, st), "moe_int4_forward");
   p.err = err ? err : w.err;
   if (int4_plan_fits(n_entries, E)) {
     cudaError_t e = launch_int4_plan(expert_indices, token_indices, n_entries, T, K, E, expert_frequency, w.off, w.s_rev,

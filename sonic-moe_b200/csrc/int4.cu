@@ -725,9 +725,17 @@ cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int
 // Row tiles of a warp's item: 2 (8 tokens, 4096 x 1024: 107 us; 1: 140 us, 4: 118 us).
 constexpr int kMT = 2;
 
-// Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice.  At 8 / 9 tokens
-// of the 4096 x 1024 layer with 128 experts this path takes 107 / 118 us, the other 117 / 120.
-bool int4_small(int T, int n_entries) { return T <= 8 && n_entries <= kSmMaxEntries; }
+// Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice.  With groups of
+// 64 or 128 this path then is the faster one (us, this / the other; 1, 4 and 8 tokens): 128 experts of 4096 x
+// 1024 29 / 40, 63 / 78, 112 / 116; 2048 x 768 at 4 and 8 34 / 45, 52 / 60; 64 experts of 7168 x 2048 58 / 70,
+// 185 / 168, 238 / 254.  Groups of 32 cost its warps more, since every group's sum is scaled apart: the other
+// path wins from about 2 10^8 weights a matrix on (4096 x 1024 at 6 and 8 tokens, 2.0 and 2.7 10^8: 100 / 102,
+// 128 / 116; 7168 x 2048 at 2 and 4, 2.3 and 4.7 10^8: 118 / 115, 210 / 167).
+bool int4_small(const Int4Args& p) {
+  if (p.T > 8 || p.n_entries > kSmMaxEntries) return false;
+  const size_t weights = static_cast<size_t>(p.n_entries < p.E ? p.n_entries : p.E) * p.H * p.I;
+  return (p.group1 > 32 && p.group2 > 32) || weights <= (size_t{3} << 26);
+}
 
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st) {
   SmallArgs u{};

@@ -31,6 +31,8 @@
 // What bounds it (512 tokens, 64 experts of 4096 x 1024): the dequantising warps.  Per SM a step of 256
 // rows takes about 1000 cycles, against 790 for its bytes at the HBM rate and 512 for its MMAs; 7 of the 11
 // instructions for 8 weights are integer ones, which an SM issues at half rate (448 cycles of the step).
+// The schedulers issue in 62% of the cycles, the integer pipe is busy in 57% of them.  24 dequantising warps
+// gain nothing (16 tokens 167 against 163 us, 64 tokens 235 against 228).
 // Fetching the codes by bulk copies from a warp of their own instead of per-lane copies, which takes a
 // tenth of the instructions away but adds a barrier wait to every step, measured 117 us against 104 (up
 // projection); double-buffered accumulators instead of the third stage of weights 239 against 228 us
@@ -659,8 +661,10 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   d.n_tiles = int4_row_tiles(d.N);
   d.k_blocks = int4_col_blocks(p.I);
   d.m_tiles = ceil_div(d.N, 256);
-  // items of 128 tokens once the experts have 32 on average (512 tokens zipf 319 us against 327, 1024 tokens
-  // 344 against 439; below, the missing overlap of the epilogue costs 2 to 4%)
+  // Items of 128 tokens once the experts have 32 on average.  4096 x 1024, 128 experts, us with 128 / 64: 512
+  // tokens even 280 / 278, Zipf 292 / 314; 1024 tokens 327 / 400 and 373 / 418; 256 tokens 245 / 246 and 259 /
+  // 267.  2048 x 768: 512 tokens 138 / 135 and 139 / 145, 256 tokens 120 / 122 and 122 / 121.  A layer with
+  // fewer items than SMs loses its share of them (40 experts of 1000 x 408, 512 tokens: 45 / 43).
   const bool many = p.n_entries >= 32 * p.E;
   e = many ? launch_wide<true, 128>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st)
            : launch_wide<true, 64>(u, p.xs, int4_padded(p.H), p.n_entries, p.group1, st);

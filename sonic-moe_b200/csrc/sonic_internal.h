@@ -127,7 +127,7 @@ cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int 
                              int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
                              bool clear_err, cudaStream_t st);
 // Few tokens: no routing plan (freq is written; off, s_rev, x_gather, tok_off, xs, y unused; err may be null).
-bool int4_small(int T, int n_entries);
+bool int4_small(const Int4Args& p);
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st);
 
 struct GemmArgs {

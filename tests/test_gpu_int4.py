@@ -116,6 +116,23 @@ def test_layer_topk(ops, T, H, I, E, K, group, concat, skew):
     assert torch.equal(out, again)  # the same bits every time
 
 
+@pytest.mark.parametrize("T", [6, 7])
+def test_few_tokens_of_a_large_layer(ops, T):
+    """Either side of the size from which a few tokens on groups of 32 take the path for many."""
+    H, I, E, K = 4096, 1024, 64, 8
+    w1, w2, g = _weights(E, H, I, T)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    idx = torch.arange(T * K, device="cuda", dtype=torch.int32).reshape(T, K).contiguous()
+    scores = torch.rand(T, K, generator=g, device="cuda") + 0.1
+    p1, p2 = ops.weight_prep_int4(w1, 32), ops.weight_prep_int4(w2, 32)
+    out, _ = ops.moe_int4_forward(x, scores, idx, p1, p2)
+    # the tokens' experts are all different: the last token's alone, as a layer of its own
+    e = slice((T - 1) * K, T * K)
+    ref, bound = oint4.experts(x[-1:], scores[-1], torch.zeros(K, device="cuda"), torch.arange(K, device="cuda"),
+                               oint4.values(w1[e], 32), oint4.values(w2[e], 32), False)
+    _check(out[-1:], ref, bound)
+
+
 @pytest.mark.parametrize("T,H,I,E,n", [(1, 128, 64, 4, 1), (1, 256, 64, 3, 9), (5, 72, 40, 3, 4), (40, 512, 256, 8, 133),
                                        (64, 256, 128, 70, 500), (8, 512, 256, 4, 256), (8, 512, 256, 4, 257), (200, 264, 136, 5, 700), (900, 128, 64, 6, 2500)])
 def test_layer_lists(ops, T, H, I, E, n):
