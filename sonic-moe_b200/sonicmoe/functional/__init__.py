@@ -506,9 +506,13 @@ class _SwitchLossFunction(torch.autograd.Function):
             return None, None, None, None
         router_logits, coef, token_mask = ctx.saved_tensors
         if torch.is_grad_enabled():  # create_graph: the same formula in operations autograd can follow
-            p = F.softmax(router_logits, dim=-1, dtype=torch.float32)
-            if token_mask is not None:
-                p = p.where(token_mask[:, None] != 0, 0.0)
+            z, on = router_logits, None
+            if token_mask is not None:  # what a left-out row holds must not reach the second gradient either
+                on = token_mask[:, None] != 0
+                z = z.where(on, 0.0)
+            p = F.softmax(z, dim=-1, dtype=torch.float32)
+            if on is not None:
+                p = p.where(on, 0.0)
             dl = dloss * p * (coef - (p * coef).sum(-1, keepdim=True))
             return dl.to(router_logits.dtype), None, None, None
         return ops.switch_loss_bwd(router_logits, coef, dloss.to(torch.float32), token_mask), None, None, None

@@ -191,6 +191,24 @@ def test_second_derivative(fn):
     assert (got.double() - want).norm() <= 1e-4 * want.norm()
 
 
+def test_second_derivative_of_left_out_rows(fn):
+    """Infinities and NaN in rows that do not count reach neither gradient."""
+    z, idx, mask = _case(30, 12, 2, torch.float32, 2, True)
+    assert not mask.all()
+    second = []
+    for fill in (None, float("nan"), float("inf")):
+        leaf = z.clone()
+        if fill is not None:
+            leaf[~mask] = fill
+        leaf.requires_grad_()
+        loss, _ = fn.switch_load_balancing_loss(leaf, topk_indices=idx, token_mask=mask)
+        (dl,) = torch.autograd.grad(loss, leaf, create_graph=True)
+        (got,) = torch.autograd.grad(dl.square().sum(), leaf)
+        assert (dl[~mask] == 0).all() and (got[~mask] == 0).all()
+        second.append(got)
+    assert torch.equal(second[0], second[1]) and torch.equal(second[0], second[2])
+
+
 def test_graph_replays_and_streams(fn):
     """Two captured graphs with their own tensors, replayed in turn on other inputs, and two streams at
     once: the results are the eager ones."""
