@@ -713,9 +713,23 @@ def weight_prep_int4(w: torch.Tensor, group_size: int = 128, concat_glu: bool = 
     return Int4ExpertWeights(q, scales, (E, N, K), group_size, bool(concat_glu))
 
 
+def _check_int4(w: Int4ExpertWeights, name: str):
+    """The prepared weight's buffers have the sizes that its shape and group need."""
+    _need(w.q, name, torch.uint8)
+    _need(w.scales, f"{name}'s scales", torch.bfloat16)
+    E, N, K = w.shape
+    blocks = E * -(-N // 16) * -(-K // 128)
+    if w.group_size not in (32, 64, 128) or w.q.numel() != 1024 * blocks or \
+            w.scales.numel() != 16 * (128 // w.group_size) * blocks:
+        raise ValueError(f"{name}: {w.q.numel()} bytes of codes and {w.scales.numel()} scales do not make a 4-bit "
+                         f"weight {tuple(w.shape)} with a group of {w.group_size}")
+
+
 def int4_expand(w: Int4ExpertWeights) -> torch.Tensor:
     """The bf16 weights [E, N, K] that a prepared 4-bit weight stands for, exactly (for a long prompt:
     ``weight_prep`` of them gives the FP8 engine's weights)."""
+    _check_int4(w, "w")
+    _same_device(w.q, scales=w.scales)
     E, N, K = w.shape
     out = torch.empty(E, N, K, dtype=torch.bfloat16, device=w.q.device)
     _call_on(out.device, "sm_int4_expand", _ptr(w.q), _ptr(w.scales), E, N, K, w.group_size, int(w.concat_glu),
@@ -736,8 +750,10 @@ def _moe_int4(x, scores, token_indices, expert_indices, n_entries, K, w1, w2, ou
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w1 {w1.shape}, w2 {w2.shape}")
     if w2.concat_glu:
         raise ValueError("w2 was prepared with concat_glu")
-    _same_device(x, scores=scores, token_indices=token_indices, expert_indices=expert_indices, w1=w1.q, w2=w2.q,
-                 out=out, expert_frequency=expert_frequency, err=err)
+    _check_int4(w1, "w1")
+    _check_int4(w2, "w2")
+    _same_device(x, scores=scores, token_indices=token_indices, expert_indices=expert_indices, w1=w1.q,
+                 w1_scales=w1.scales, w2=w2.q, w2_scales=w2.scales, out=out, expert_frequency=expert_frequency, err=err)
     dev = x.device
     if out is None:
         out = torch.empty(T, H, dtype=torch.bfloat16, device=dev)

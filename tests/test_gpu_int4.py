@@ -149,7 +149,7 @@ def test_layer_lists(ops, T, H, I, E, n):
     _check(out, ref, bound)
 
 
-@pytest.mark.parametrize("T", [4, 60, 400])
+@pytest.mark.parametrize("T", [4, 60, 400, 8300])
 def test_bad_entries_are_reported_and_left_out(ops, T):
     E, H, I, K = 6, 256, 64, 2
     w1, w2, g = _weights(E, H, I, T)
@@ -313,3 +313,21 @@ def test_module_runs_both_operators(ops):
     m.eval().use_int4_experts(None)
     back, _ = m(x, is_inference_mode=True)
     assert (back - fp8).abs().max() <= 2.0 ** -6 * fp8.abs().max()  # bf16 sums in any order, as before
+
+
+def test_prepared_buffers_are_checked(ops):
+    """Buffers that do not belong to the shape and the group are refused before anything runs."""
+    import dataclasses
+
+    w1, w2, g = _weights(2, 128, 64, 0)
+    p1, p2 = ops.weight_prep_int4(w1, 32), ops.weight_prep_int4(w2, 32)
+    x = torch.randn(3, 128, generator=g, device="cuda").to(torch.bfloat16)
+    idx, scores = _routing(3, 2, 1, g)
+    for change in (dict(q=p1.q[:-16]), dict(scales=p1.scales[:-8]), dict(group_size=64), dict(group_size=0),
+                   dict(scales=p1.scales.cpu()), dict(q=p1.q.cpu()), dict(q=p1.q.to(torch.int32)),
+                   dict(scales=p1.scales.float()), dict(shape=(4, 128, 128))):
+        bad = dataclasses.replace(p1, **change)
+        with pytest.raises(ValueError):
+            ops.moe_int4_forward(x, scores, idx, bad, p2)
+        with pytest.raises(ValueError):
+            ops.int4_expand(bad)
