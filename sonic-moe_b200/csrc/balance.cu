@@ -90,44 +90,95 @@ __device__ __forceinline__ void store8(InT* __restrict__ dst, int vec, int n, co
     if (j < n) dst[j] = raw[j];
 }
 
-// Reductions over the L lanes that share a row: lanes of one warp (L <= 32) or the whole CTA, whose
-// partial results go through s_red.  Every thread of the group gets the result.
-template <int L, bool kMax>
-__device__ __forceinline__ float row_reduce(float x, float* s_red) {
+// Two fp32 operations in one instruction, each half rounded as the scalar operation would.
+__device__ __forceinline__ unsigned long long f2_bits(float2 v) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 f2_of(unsigned long long b) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b));
+  return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_of(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return f2_of(r);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// N reductions at once over the L lanes that share a row: lanes of one warp (L <= 32) or the whole CTA,
+// whose partial results go through s_red [N * L / 32].  Every thread of the group gets the results.
+template <int L, bool kMax, int N>
+__device__ __forceinline__ void row_reduce(float (&x)[N], float* s_red) {
 #pragma unroll
-  for (int o = (L < 32 ? L : 32) / 2; o >= 1; o >>= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, x, o);
-    x = kMax ? fmaxf(x, y) : x + y;
-  }
+  for (int o = (L < 32 ? L : 32) / 2; o >= 1; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float y = __shfl_xor_sync(0xffffffffu, x[n], o);
+      x[n] = kMax ? fmaxf(x[n], y) : x[n] + y;
+    }
   if constexpr (L > 32) {
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = s_red[0];
+    if ((threadIdx.x & 31) == 0)
 #pragma unroll
-    for (int w = 1; w < L / 32; ++w) x = kMax ? fmaxf(x, s_red[w]) : x + s_red[w];
+      for (int n = 0; n < N; ++n) s_red[n * (L / 32) + (threadIdx.x >> 5)] = x[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      x[n] = s_red[n * (L / 32)];
+#pragma unroll
+      for (int w = 1; w < L / 32; ++w) {
+        const float y = s_red[n * (L / 32) + w];
+        x[n] = kMax ? fmaxf(x[n], y) : x[n] + y;
+      }
+    }
   }
-  return x;
 }
 
-// The softmax of one row held as 8 * C values a lane: v becomes exp2(log2e (x - max)), the return
-// value 1 / sum.  The maximum is subtracted before the scaling, so that a row of the type's lowest
-// values does not overflow.  A row whose maximum is not finite (all -inf, or +inf or NaN in it) gives
-// NaN, as a softmax does.
-template <int L, int C>
-__device__ __forceinline__ float softmax_row(float (&v)[8 * C], float* s_red) {
-  float mx = v[0];
+// R rows held as 8 * C values a lane: v becomes exp2(log2e (x - max)), s the lane's sum of it.  The
+// maximum is subtracted before the scaling, so that a row of the type's lowest values does not overflow.
+// A row whose maximum is not finite (all -inf, or +inf or NaN in it) gives NaN, as a softmax does.
+template <int L, int C, int R>
+__device__ __forceinline__ void exp_rows(float2 (&v)[R][4 * C], float (&s)[R], float* s_red) {
+  float mx[R];
 #pragma unroll
-  for (int i = 1; i < 8 * C; ++i) mx = fmaxf(mx, v[i]);
-  mx = row_reduce<L, true>(mx, s_red);
-  float s = 0.0f;
+  for (int j = 0; j < R; ++j) {
+    mx[j] = fmaxf(v[j][0].x, v[j][0].y);
 #pragma unroll
-  for (int i = 0; i < 8 * C; ++i) {
-    v[i] = ex2((v[i] - mx) * kLog2e);
-    s += v[i];
+    for (int i = 1; i < 4 * C; ++i) mx[j] = fmaxf(mx[j], fmaxf(v[j][i].x, v[j][i].y));
   }
-  return 1.0f / row_reduce<L, false>(s, s_red);
+  row_reduce<L, true, R>(mx, s_red);
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    float2 s2 = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < 4 * C; ++i) {
+      const float2 t = mul2(add2(v[j][i], both(-mx[j])), both(kLog2e));
+      v[j][i] = make_float2(ex2(t.x), ex2(t.y));
+      s2 = add2(s2, v[j][i]);
+    }
+    s[j] = s2.x + s2.y;
+  }
 }
+// 1 / s of a row's sum, 1 <= s <= E: within two units in the last place.
+__device__ __forceinline__ float row_inv(float s) { return __fdividef(1.0f, s); }
+
+// Rows that a group takes at once: two, where the registers allow it, keep twice the loads on the way and
+// fill the latencies of one row's reductions with the other's.
+template <int C>
+constexpr int kRows = C == 1 ? 2 : 1;
 
 // Lane layout: group lane l holds columns 8 l + 8 L c + (0..7), c < C; E <= 8 L C.  A row that does not
 // count is not read (zeros stand in).
@@ -145,9 +196,10 @@ __device__ __forceinline__ void load_row(const InT* __restrict__ row, bool on, i
   }
 }
 template <typename InT, int C>
-__device__ __forceinline__ void row_f32(const Raw8<InT> (&raw)[C], float (&v)[8 * C]) {
+__device__ __forceinline__ void row_f32(const Raw8<InT> (&raw)[C], float2 (&v)[4 * C]) {
 #pragma unroll
-  for (int i = 0; i < 8 * C; ++i) v[i] = to_f32(raw[i / 8].v[i % 8]);
+  for (int i = 0; i < 4 * C; ++i)
+    v[i] = make_float2(to_f32(raw[i / 4].v[2 * i % 8]), to_f32(raw[i / 4].v[2 * i % 8 + 1]));
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -220,36 +272,57 @@ __global__ void __launch_bounds__(kSlThreads)
   constexpr int kGroups = kSlThreads / L;               // rows of a CTA's step
   constexpr int kCopies = L < 32 ? kSlThreads / 32 : kGroups;
   extern __shared__ float s_dyn[];
-  __shared__ float s_red[8];
+  __shared__ float s_red[16 * kRows<C>];
   float* s_p = s_dyn;
   int32_t* s_f = reinterpret_cast<int32_t*>(s_dyn + static_cast<size_t>(kCopies) * E);
   const int gl = threadIdx.x % L, grp = threadIdx.x / L;
   pdl_launch();
   if (idx)
     for (int e = threadIdx.x; e < E; e += kSlThreads) s_f[e] = 0;
-  float acc[8 * C];
+  float2 acc2[4 * C];
 #pragma unroll
-  for (int i = 0; i < 8 * C; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < 4 * C; ++i) acc2[i] = both(0.0f);
   // every group takes the same number of rows, so that the shuffles and barriers below are uniform; the
-  // next row is under way while one is reduced
+  // next rows are under way while some are reduced
+  constexpr int R = kRows<C>;
   const long long stride = static_cast<long long>(gridDim.x) * kGroups;
   auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
   long long r = static_cast<long long>(blockIdx.x) * kGroups + grp;
-  Raw8<InT> next[C];
-  bool on_next = counts(r);
-  load_row<InT, L, C>(logits + r * E, on_next, E, vec, gl, next);
-  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += stride) {
-    float v[8 * C];
-    row_f32<InT, C>(next, v);
-    const bool on = on_next;
-    r += stride;
-    on_next = counts(r);
-    load_row<InT, L, C>(logits + r * E, on_next, E, vec, gl, next);
-    const float inv = softmax_row<L, C>(v, s_red);
-    if (on) {
+  Raw8<InT> next[R][C];
+  bool on_next[R];
+  auto load = [&] {
 #pragma unroll
-      for (int i = 0; i < 8 * C; ++i) acc[i] = fmaf(v[i], inv, acc[i]);
+    for (int j = 0; j < R; ++j) on_next[j] = counts(r + j * stride);
+#pragma unroll
+    for (int j = 0; j < R; ++j) load_row<InT, L, C>(logits + (r + j * stride) * E, on_next[j], E, vec, gl, next[j]);
+  };
+  load();
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += R * stride) {
+    float2 v[R][4 * C];
+    bool on[R];
+    float sum[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      row_f32<InT, C>(next[j], v[j]);
+      on[j] = on_next[j];
     }
+    r += R * stride;
+    load();
+    exp_rows<L, C, R>(v, sum, s_red);
+    row_reduce<L, false, R>(sum, s_red);
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (on[j]) {
+        const float2 inv = both(row_inv(sum[j]));
+#pragma unroll
+        for (int i = 0; i < 4 * C; ++i) acc2[i] = fma2(v[j][i], inv, acc2[i]);
+      }
+  }
+  float acc[8 * C];
+#pragma unroll
+  for (int i = 0; i < 4 * C; ++i) {
+    acc[2 * i] = acc2[i].x;
+    acc[2 * i + 1] = acc2[i].y;
   }
   // rows of one warp first (lanes that hold the same columns), then the warps through shared memory
   if constexpr (L < 32) {
@@ -354,43 +427,70 @@ __global__ void __launch_bounds__(kSlThreads)
                            const float* __restrict__ coef, const float* __restrict__ dloss,
                            InT* __restrict__ dlogits) {
   constexpr int kGroups = kSlThreads / L;
-  __shared__ float s_red[8];
+  __shared__ float s_red[16 * kRows<C>];
   const int gl = threadIdx.x % L, grp = threadIdx.x / L;
   const float g = *dloss;
-  float c[8 * C];
+  float2 c[4 * C];
 #pragma unroll
-  for (int k = 0; k < C; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int e = 8 * gl + 8 * L * k + j;
-      c[8 * k + j] = e < E ? coef[e] : 0.0f;
-    }
+  for (int i = 0; i < 4 * C; ++i) {
+    const int e = 8 * gl + 8 * L * (i / 4) + 2 * (i % 4);
+    c[i] = make_float2(e < E ? coef[e] : 0.0f, e + 1 < E ? coef[e + 1] : 0.0f);
+  }
+  constexpr int R = kRows<C>;
   const long long stride = static_cast<long long>(gridDim.x) * kGroups;
   auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
-  long long r_next = static_cast<long long>(blockIdx.x) * kGroups + grp;
-  Raw8<InT> next[C];
-  bool on_next = counts(r_next);
-  load_row<InT, L, C>(logits + r_next * E, on_next, E, vec, gl, next);
-  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += stride) {
-    float v[8 * C];
-    row_f32<InT, C>(next, v);
-    const long long r = r_next;
-    const bool on = on_next;
-    r_next += stride;
-    on_next = counts(r_next);
-    load_row<InT, L, C>(logits + r_next * E, on_next, E, vec, gl, next);
-    const float inv = softmax_row<L, C>(v, s_red);
-    float dot = 0.0f;
+  long long r = static_cast<long long>(blockIdx.x) * kGroups + grp;
+  Raw8<InT> next[R][C];
+  bool on_next[R];
+  auto load = [&](long long at) {
 #pragma unroll
-    for (int i = 0; i < 8 * C; ++i) dot = fmaf(v[i], c[i], dot);
-    dot = row_reduce<L, false>(dot, s_red) * inv;
-    if (r >= T) continue;
-    // a token that does not count gets a gradient of exactly 0, whatever its logits hold
+    for (int j = 0; j < R; ++j) on_next[j] = counts(at + j * stride);
 #pragma unroll
-    for (int i = 0; i < 8 * C; ++i) v[i] = on ? g * (v[i] * inv * (c[i] - dot)) : 0.0f;
+    for (int j = 0; j < R; ++j) load_row<InT, L, C>(logits + (at + j * stride) * E, on_next[j], E, vec, gl, next[j]);
+  };
+  load(r);
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kGroups; r0 < T; r0 += R * stride, r += R * stride) {
+    float2 v[R][4 * C];
+    bool on[R];
+    float sum[R], sums[2 * R];  // the rows' sums, then their products with c
 #pragma unroll
-    for (int k = 0; k < C; ++k)
-      store8<InT>(dlogits + r * E + 8 * gl + 8 * L * k, vec, E - 8 * gl - 8 * L * k, v + 8 * k);
+    for (int j = 0; j < R; ++j) {
+      row_f32<InT, C>(next[j], v[j]);
+      on[j] = on_next[j];
+    }
+    load(r + R * stride);
+    exp_rows<L, C, R>(v, sum, s_red);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float2 d = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < 4 * C; ++i) d = fma2(v[j][i], c[i], d);
+      sums[j] = sum[j];
+      sums[R + j] = d.x + d.y;
+    }
+    row_reduce<L, false, 2 * R>(sums, s_red);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const long long row = r + j * stride;
+      if (row >= T) continue;
+      float w[8 * C];
+      if (on[j]) {
+        const float inv = row_inv(sums[j]);
+        const float2 gi = both(g * inv), dot = both(-sums[R + j] * inv);
+#pragma unroll
+        for (int i = 0; i < 4 * C; ++i) {
+          const float2 o = mul2(mul2(v[j][i], gi), add2(c[i], dot));
+          w[2 * i] = o.x;
+          w[2 * i + 1] = o.y;
+        }
+      } else {  // a token that does not count gets a gradient of exactly 0, whatever its logits hold
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i) w[i] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        store8<InT>(dlogits + row * E + 8 * gl + 8 * L * k, vec, E - 8 * gl - 8 * L * k, w + 8 * k);
+    }
   }
 }
 
