@@ -122,13 +122,18 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // whose partial results go through s_red [N * L / 32].  Every thread of the group gets the results.
 template <int L, bool kMax, int N>
 __device__ __forceinline__ void row_reduce(float (&x)[N], float* s_red) {
+  if constexpr (L >= 32 && kMax) {  // one instruction for a warp's maximum
 #pragma unroll
-  for (int o = (L < 32 ? L : 32) / 2; o >= 1; o >>= 1)
+    for (int n = 0; n < N; ++n) asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(x[n]) : "f"(x[n]));
+  } else {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const float y = __shfl_xor_sync(0xffffffffu, x[n], o);
-      x[n] = kMax ? fmaxf(x[n], y) : x[n] + y;
-    }
+    for (int o = (L < 32 ? L : 32) / 2; o >= 1; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float y = __shfl_xor_sync(0xffffffffu, x[n], o);
+        x[n] = kMax ? fmaxf(x[n], y) : x[n] + y;
+      }
+  }
   if constexpr (L > 32) {
     __syncthreads();
     if ((threadIdx.x & 31) == 0)
@@ -176,9 +181,10 @@ __device__ __forceinline__ void exp_rows(float2 (&v)[R][4 * C], float (&s)[R], f
 __device__ __forceinline__ float row_inv(float s) { return __fdividef(1.0f, s); }
 
 // Rows that a group takes at once: two, where the registers allow it, keep twice the loads on the way and
-// fill the latencies of one row's reductions with the other's.
-template <int C>
-constexpr int kRows = C == 1 ? 2 : 1;
+// fill the latencies of one row's reductions with the other's (131072 x 256: forward 35 us against 39,
+// backward 27 against 31).  An fp32 row of a whole warp has as many bytes by itself (42 us against 47).
+template <typename InT, int L, int C>
+constexpr int kRows = C == 1 && (sizeof(InT) == 2 || L < 32) ? 2 : 1;
 
 // Lane layout: group lane l holds columns 8 l + 8 L c + (0..7), c < C; E <= 8 L C.  A row that does not
 // count is not read (zeros stand in).
@@ -203,8 +209,14 @@ __device__ __forceinline__ void row_f32(const Raw8<InT> (&raw)[C], float2 (&v)[4
 }
 
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
 }
 // The 32-bit word at this CTA's shared address `p`, in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t ld_cluster(const void* p, int rank) {
@@ -214,52 +226,86 @@ __device__ __forceinline__ uint32_t ld_cluster(const void* p, int rank) {
   return v;
 }
 
-// Loss and gradient coefficients from the column sums: thread i of the CTA calls with every e it owns.
-__device__ __forceinline__ float block_sum(float x, float* s_red) {
+// The threads' x and f summed over the CTA, in a fixed order; every thread gets the sums.
+struct FinishSums {
+  float x[32];
+  long long f[32];
+};
+__device__ __forceinline__ void block_sums(float& x, long long& f, FinishSums& sm) {
   __syncthreads();
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
+  for (int o = 16; o >= 1; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    f += __shfl_xor_sync(0xffffffffu, f, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sm.x[threadIdx.x >> 5] = x;
+    sm.f[threadIdx.x >> 5] = f;
+  }
   __syncthreads();
-  float r = 0.0f;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) r += s_red[w];
-  return r;
-}
-__device__ __forceinline__ long long block_sum_int(long long x, long long* s_red) {
-  __syncthreads();
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  long long r = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) r += s_red[w];
-  return r;
+  x = 0.0f;
+  f = 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
+    x += sm.x[w];
+    f += sm.f[w];
+  }
 }
 
-// P (column sums) and f (counts) of all experts in shared memory -> loss, c, counts.
-__device__ void finish(const float* s_p, const int32_t* s_f, int E, float* __restrict__ loss,
+// P (column sums) and f (counts) of the CTA's experts e0 .. e0 + n_own - 1 in shared memory -> loss, c,
+// counts.  kClustered: the CTAs of a cluster hold the experts between them.
+template <bool kClustered>
+__device__ void finish(const float* s_p, const int32_t* s_f, int E, int e0, int n_own, float* __restrict__ loss,
                        float* __restrict__ coef, int32_t* __restrict__ freq_out) {
-  __shared__ float s_red[32];
-  __shared__ long long s_redi[32];
-  float p = 0.0f;
-  long long f = 0;
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    p += s_p[e];
-    f += s_f[e];
+  __shared__ FinishSums s_sums;
+  __shared__ float s_x[2];  // the CTA's sum of P, its part of the loss
+  __shared__ int32_t s_count[2];
+  float n = 0.0f;
+  long long F = 0;
+  for (int e = threadIdx.x; e < n_own; e += blockDim.x) {
+    n += s_p[e];
+    F += s_f[e];
   }
-  const float n = block_sum(p, s_red);
-  const long long F = block_sum_int(f, s_redi);
+  block_sums(n, F, s_sums);
+  if constexpr (kClustered) {
+    if (threadIdx.x == 0) {
+      s_x[0] = n;
+      s_count[0] = static_cast<int32_t>(F & 0xffffffff);
+      s_count[1] = static_cast<int32_t>(F >> 32);
+    }
+    cluster_sync();
+    n = 0.0f;
+    F = 0;
+#pragma unroll
+    for (int k = 0; k < kSlCluster; ++k) {
+      n += __uint_as_float(ld_cluster(&s_x[0], k));
+      F += static_cast<long long>(static_cast<unsigned long long>(ld_cluster(&s_count[1], k)) << 32 |
+                                  ld_cluster(&s_count[0], k));
+    }
+  }
   // no token counts, or no entry: the loss and the gradient are 0 (a NaN sum stays NaN)
   const float inv_n = n == 0.0f ? 0.0f : 1.0f / n;
   const float inv_f = F == 0 ? 0.0f : 1.0f / static_cast<float>(F);
   float l = 0.0f;
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+  for (int e = threadIdx.x; e < n_own; e += blockDim.x) {
     l += (s_p[e] * inv_n) * (static_cast<float>(s_f[e]) * inv_f);
-    coef[e] = static_cast<float>(static_cast<long long>(s_f[e]) * E - F) * inv_f * inv_n;
-    if (freq_out) freq_out[e] = s_f[e];
+    coef[e0 + e] = static_cast<float>(static_cast<long long>(s_f[e]) * E - F) * inv_f * inv_n;
+    if (freq_out) freq_out[e0 + e] = s_f[e];
   }
-  l = block_sum(l, s_red);
-  if (threadIdx.x == 0) *loss = l * static_cast<float>(E);
+  long long none = 0;
+  block_sums(l, none, s_sums);
+  if constexpr (kClustered) {
+    if (threadIdx.x == 0) s_x[1] = l;
+    cluster_sync();
+    if (cluster_rank() == 0) {
+      l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSlCluster; ++k) l += __uint_as_float(ld_cluster(&s_x[1], k));
+      if (threadIdx.x == 0) *loss = l * static_cast<float>(E);
+    }
+    cluster_sync();  // nobody's shared memory goes away while it is read
+  } else {
+    if (threadIdx.x == 0) *loss = l * static_cast<float>(E);
+  }
 }
 
 // Dynamic shared memory: column sums [kSlThreads / max(L, 32)][E] (one copy per warp, or one), counts [E].
@@ -272,7 +318,7 @@ __global__ void __launch_bounds__(kSlThreads)
   constexpr int kGroups = kSlThreads / L;               // rows of a CTA's step
   constexpr int kCopies = L < 32 ? kSlThreads / 32 : kGroups;
   extern __shared__ float s_dyn[];
-  __shared__ float s_red[16 * kRows<C>];
+  __shared__ float s_red[16 * kRows<InT, L, C>];
   float* s_p = s_dyn;
   int32_t* s_f = reinterpret_cast<int32_t*>(s_dyn + static_cast<size_t>(kCopies) * E);
   const int gl = threadIdx.x % L, grp = threadIdx.x / L;
@@ -284,7 +330,7 @@ __global__ void __launch_bounds__(kSlThreads)
   for (int i = 0; i < 4 * C; ++i) acc2[i] = both(0.0f);
   // every group takes the same number of rows, so that the shuffles and barriers below are uniform; the
   // next rows are under way while some are reduced
-  constexpr int R = kRows<C>;
+  constexpr int R = kRows<InT, L, C>;
   const long long stride = static_cast<long long>(gridDim.x) * kGroups;
   auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
   long long r = static_cast<long long>(blockIdx.x) * kGroups + grp;
@@ -362,7 +408,7 @@ __global__ void __launch_bounds__(kSlThreads)
   }
   if (gridDim.x == 1) {
     __syncthreads();
-    finish(s_p, s_f, E, loss, coef, freq_out);
+    finish<false>(s_p, s_f, E, 0, E, loss, coef, freq_out);
     return;
   }
   // the cluster's CTAs each add an eighth of the columns over all 8
@@ -383,42 +429,48 @@ __global__ void __launch_bounds__(kSlThreads)
   cluster_sync();  // nobody's shared memory goes away while it is read
 }
 
-// The clusters' sums, `slices` groups of threads each adding every slices-th part, then the groups in order.
+// The clusters' sums: `slices` groups of threads each add every slices-th part, then the groups are added in
+// order.  Up to 256 experts one CTA does it; more are shared by the CTAs of a cluster, since the chain of
+// loads would take longer than its barriers (forward, us, one CTA / a cluster: 20000 x 4096 138 / 82, 65536 x
+// 512 37 / 34, 131072 x 256 35 / 35, 32768 x 128 14 / 16).
 constexpr int kFinThreads = 1024;
-constexpr int kFinSlots = 4096;  // slices * E <= kFinSlots
+constexpr int kFinOneCta = 256;
 
+template <bool kClustered>
 __global__ void __launch_bounds__(kFinThreads)
     switch_loss_finish_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_f, int parts, int E,
                               int slices, const int32_t* __restrict__ freq_in, float* __restrict__ loss,
                               float* __restrict__ coef, int32_t* __restrict__ freq_out) {
-  __shared__ float s_p[kFinSlots];
-  __shared__ int32_t s_f[kFinSlots];
+  __shared__ float s_p[kFinThreads];
+  __shared__ int32_t s_f[kFinThreads];
+  const int own = kClustered ? (E + kSlCluster - 1) / kSlCluster : E;  // slices * own <= kFinThreads
+  const int e0 = kClustered ? min(E, cluster_rank() * own) : 0, n_own = min(own, E - e0);
+  const int sl = threadIdx.x / own, c = threadIdx.x - sl * own;
   pdl_wait();
-  for (int i = threadIdx.x; i < slices * E; i += kFinThreads) {
-    const int sl = i / E, e = i - sl * E;
+  if (sl < slices && c < n_own) {
     float p = 0.0f;
     int f = 0;
-#pragma unroll 8
+#pragma unroll 12
     for (int k = sl; k < parts; k += slices) {
-      p += part_p[static_cast<size_t>(k) * E + e];
-      if (part_f) f += part_f[static_cast<size_t>(k) * E + e];
+      p += part_p[static_cast<size_t>(k) * E + e0 + c];
+      if (part_f) f += part_f[static_cast<size_t>(k) * E + e0 + c];
     }
-    s_p[i] = p;
-    s_f[i] = f;
+    s_p[threadIdx.x] = p;
+    s_f[threadIdx.x] = f;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kFinThreads) {
-    float p = s_p[e];
-    int f = s_f[e];
-    for (int sl = 1; sl < slices; ++sl) {
-      p += s_p[sl * E + e];
-      f += s_f[sl * E + e];
+  if (threadIdx.x < n_own) {
+    float p = s_p[threadIdx.x];
+    int f = s_f[threadIdx.x];
+    for (int k = 1; k < slices; ++k) {
+      p += s_p[k * own + threadIdx.x];
+      f += s_f[k * own + threadIdx.x];
     }
-    s_p[e] = p;
-    s_f[e] = part_f ? f : freq_in[e];
+    s_p[threadIdx.x] = p;
+    s_f[threadIdx.x] = part_f ? f : freq_in[e0 + threadIdx.x];
   }
   __syncthreads();
-  finish(s_p, s_f, E, loss, coef, freq_out);
+  finish<kClustered>(s_p, s_f, E, e0, n_own, loss, coef, freq_out);
 }
 
 template <typename InT, int L, int C>
@@ -427,7 +479,7 @@ __global__ void __launch_bounds__(kSlThreads)
                            const float* __restrict__ coef, const float* __restrict__ dloss,
                            InT* __restrict__ dlogits) {
   constexpr int kGroups = kSlThreads / L;
-  __shared__ float s_red[16 * kRows<C>];
+  __shared__ float s_red[16 * kRows<InT, L, C>];
   const int gl = threadIdx.x % L, grp = threadIdx.x / L;
   const float g = *dloss;
   float2 c[4 * C];
@@ -436,7 +488,7 @@ __global__ void __launch_bounds__(kSlThreads)
     const int e = 8 * gl + 8 * L * (i / 4) + 2 * (i % 4);
     c[i] = make_float2(e < E ? coef[e] : 0.0f, e + 1 < E ? coef[e + 1] : 0.0f);
   }
-  constexpr int R = kRows<C>;
+  constexpr int R = kRows<InT, L, C>;
   const long long stride = static_cast<long long>(gridDim.x) * kGroups;
   auto counts = [&](long long r) { return r < T && (!mask || mask[r]); };
   long long r = static_cast<long long>(blockIdx.x) * kGroups + grp;
@@ -556,10 +608,11 @@ cudaError_t launch_lc(const SlArgs& a, bool bwd, cudaStream_t st) {
   e = cudaLaunchKernelEx(&cfg, kern, x, a.T, a.E, vec, a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss, a.coef,
                          a.freq_out, a.err);
   if (e != cudaSuccess) return e;
-  const int slices = a.E >= kFinThreads ? 1 : kFinThreads / a.E;
-  return launch_dependent(switch_loss_finish_kernel, dim3(1), kFinThreads, 0, 1, st, a.part_p,
-                          a.idx ? a.part_f : nullptr, a.grid, a.E, slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef,
-                          a.freq_out);
+  const bool one = a.E <= kFinOneCta;
+  const int ctas = one ? 1 : kSlCluster, slices = kFinThreads / ceil_div(a.E, ctas);
+  return launch_dependent(one ? switch_loss_finish_kernel<false> : switch_loss_finish_kernel<true>, dim3(ctas),
+                          kFinThreads, 0, ctas, st, a.part_p, a.idx ? a.part_f : nullptr, a.grid, a.E,
+                          slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef, a.freq_out);
 }
 
 // Lanes per row: as many as hold the row at 8 values each, up to a warp; wider rows take 16 or 32
