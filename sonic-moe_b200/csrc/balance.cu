@@ -15,6 +15,12 @@
 // switch_loss_finish_kernel adds the clusters' sums in a fixed order (no floating-point atomics: the loss
 //                           is the same bits every time) and forms the loss and c.
 // switch_loss_bwd_kernel    reads the logits once more, recomputes the softmax, writes the gradient.
+//
+// 131072 x 256 bf16: forward with counts 35 us, backward 27 us, against 11 and 21 us for their bytes.  The
+// backward is bound by its instructions (76% of the issue slots; 151 a row of 256 for a warp, so operations
+// go in pairs and a maximum in one instruction), the forward by the latency of a row's two reductions
+// (54%), hence two rows a warp and the next two on the way.  Up to a few thousand tokens it is the launches:
+// one CTA 4 us, two kernels 10 us.
 #include "common.cuh"
 #include "sonic_internal.h"
 
@@ -24,7 +30,7 @@ namespace {
 
 constexpr int kSlThreads = 256;
 constexpr int kSlCluster = 8;       // CTAs of the forward that add their sums before they write them
-constexpr int kSlMaxParts = 4 * 18;  // clusters at most (148 SMs hold 18)
+constexpr int kSlMaxParts = 4 * 18;  // clusters at most: 4 CTAs per SM (5 or 6: 131072 x 256 37 us against 35)
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {

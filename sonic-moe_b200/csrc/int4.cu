@@ -725,7 +725,9 @@ cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int
 // Row tiles of a warp's item: 2 (8 tokens, 4096 x 1024: 107 us; 1: 140 us, 4: 118 us).
 constexpr int kMT = 2;
 
-// Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice.  With groups of
+// Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice; beyond, that
+// depends on the routing (4096 x 1024, 128 experts, this / the other: 16 tokens even 142 / 162, Zipf 115 / 109,
+// 24 tokens 180 / 193 and 180 / 135).  With groups of
 // 64 or 128 this path then is the faster one (us, this / the other; 1, 4 and 8 tokens): 128 experts of 4096 x
 // 1024 29 / 40, 63 / 78, 112 / 116; 2048 x 768 at 4 and 8 34 / 45, 52 / 60; 64 experts of 7168 x 2048 58 / 70,
 // 185 / 168, 238 / 254.  Groups of 32 cost its warps more, since every group's sum is scaled apart: the other
