@@ -726,13 +726,13 @@ cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int
 constexpr int kMT = 2;
 
 // Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice; beyond, that
-// depends on the routing (4096 x 1024, 128 experts, this / the other: 16 tokens even 142 / 162, Zipf 115 / 109,
-// 24 tokens 180 / 193 and 180 / 135).  With groups of
-// 64 or 128 this path then is the faster one (us, this / the other; 1, 4 and 8 tokens): 128 experts of 4096 x
-// 1024 29 / 40, 63 / 78, 112 / 116; 2048 x 768 at 4 and 8 34 / 45, 52 / 60; 64 experts of 7168 x 2048 58 / 70,
-// 185 / 168, 238 / 254.  Groups of 32 cost its warps more, since every group's sum is scaled apart: the other
-// path wins from about 2 10^8 weights a matrix on (4096 x 1024 at 6 and 8 tokens, 2.0 and 2.7 10^8: 100 / 102,
-// 128 / 116; 7168 x 2048 at 2 and 4, 2.3 and 4.7 10^8: 118 / 115, 210 / 167).
+// depends on the routing (4096 x 1024, 128 experts, us, this / the other: 16 tokens even 142 / 162, Zipf 115 /
+// 109; 24 tokens 180 / 193 and 180 / 135).  With groups of 64 or 128 this path is then the faster one but for
+// single points (1, 4 and 8 tokens of 4096 x 1024 29 / 40, 63 / 78, 112 / 116; 4 and 8 of 2048 x 768 34 / 45,
+// 52 / 60; 1, 4 and 8 of 7168 x 2048 with 64 experts 58 / 70, 185 / 168, 238 / 254).  Groups of 32 cost its
+// warps more, since every group's sum is scaled apart: the other path wins from about 2 10^8 weights a matrix
+// on (4096 x 1024 at 6 and 8 tokens, 2.0 and 2.7 10^8: 100 / 102, 128 / 116; 7168 x 2048 at 2 and 4, 2.3 and
+// 4.7 10^8: 118 / 115, 210 / 167).
 bool int4_small(const Int4Args& p) {
   if (p.T > 8 || p.n_entries > kSmMaxEntries) return false;
   const size_t weights = static_cast<size_t>(p.n_entries < p.E ? p.n_entries : p.E) * p.H * p.I;

@@ -176,7 +176,7 @@ def test_bad_entries_are_reported_and_left_out(ops, T):
     assert err.item() == 204
 
 
-@pytest.mark.parametrize("T", [9, 80])
+@pytest.mark.parametrize("T", [8, 9, 80])
 def test_infinite_and_nan_tokens_stay_in_their_rows(ops, T):
     E, H, I, K = 4, 264, 72, 2
     w1, w2, g = _weights(E, H, I, T)
