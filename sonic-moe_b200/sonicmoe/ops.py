@@ -603,7 +603,8 @@ def _same_device(first: torch.Tensor, **others):
 
 def _call_on(device: torch.device, name: str, *args):
     """Enqueue an entry point on the current stream of the tensors' device, whichever device is current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: a Stream object around it takes 2 us, a tenth of a small call
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if torch.cuda.current_device() == device.index:
         nat.call(name, *args, stream)
     else:
