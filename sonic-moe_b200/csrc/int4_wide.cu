@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(256)
     const int k = 32 * b + 8 * t;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (ok && k < K) v = __ldg(reinterpret_cast<const uint4*>(x + static_cast<size_t>(tok) * K + k));
-    // round 1: swap the 2 x 2 blocks between t and t ^ 2, round 2: within them between t and t ^ 1
+    // first swap the 2 x 2 blocks between t and t ^ 2, then within them between t and t ^ 1
     const bool hi = t & 2, odd = t & 1;
     const uint32_t s0 = __shfl_xor_sync(0xffffffffu, hi ? v.x : v.z, 2), s1 = __shfl_xor_sync(0xffffffffu, hi ? v.y : v.w, 2);
     if (hi) {
