@@ -513,7 +513,8 @@ int sm_int4_expand(const uint8_t* wq, const void* scales, int E, int N, int K, i
  *   K = 0: explicit lists of n_entries, token_indices sorted ascending.
  *   w1q / w2q: sm_weight_prep_int4 of [E, 2I, H] / [E, H, I].  H and I multiples of 8.
  * expert_frequency [E] receives the entries per expert.  An entry whose expert is outside [0, E) or
- * whose token is outside [0, T) contributes nothing and sets err (201 / 204); err may be NULL.
+ * whose token is outside [0, T) contributes nothing and sets err (201 / 204) if it was 0; err may be NULL.
+ * What err holds before the call has no influence on it.
  */
 size_t sm_moe_int4_workspace_bytes(int T, int n_entries, int H, int I, int E);
 int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_entries, const float* scores,

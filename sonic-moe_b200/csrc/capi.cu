@@ -758,7 +758,8 @@ struct Int4Ws {
   void* xs;
   void* a;
   float* y;
-  int32_t* err;
+  int32_t* err;   // stands in for the caller's error word; nobody reads it
+  int32_t* stop;  // this call's waits that gave up
 };
 
 Int4Ws carve_int4(Carve& c, int T, int n_entries, int H, int I, int E) {
@@ -773,6 +774,7 @@ Int4Ws carve_int4(Carve& c, int T, int n_entries, int H, int I, int E) {
   w.a = c.take<uint16_t>(static_cast<size_t>(n_entries) * int4_padded(I));
   w.y = c.take<float>(static_cast<size_t>(n_entries) * H);
   w.err = c.take<int32_t>(1);
+  w.stop = c.take<int32_t>(1);
   return w;
 }
 
@@ -920,14 +922,14 @@ int sm_moe_int4_forward(const void* x, int T, int H, int I, int E, int K, int n_
   p.err = err;
   if (int4_small(p)) return cuda_status(launch_int4_small(p, st), "moe_int4_forward");
   p.err = err ? err : w.err;
+  p.stop = w.stop;
   if (int4_plan_fits(n_entries, E)) {
     cudaError_t e = launch_int4_plan(expert_indices, token_indices, n_entries, T, K, E, expert_frequency, w.off, w.s_rev,
-                                     w.x_gather, w.tok_off, p.err, !err, st);
+                                     w.x_gather, w.tok_off, p.err, p.stop, st);
     if (e == cudaSuccess) e = launch_int4_wide(p, st);
     return cuda_status(e, "moe_int4_forward");
   }
-  cudaError_t e = cudaSuccess;
-  if (!err) e = cudaMemsetAsync(w.err, 0, sizeof(int32_t), st);
+  cudaError_t e = cudaMemsetAsync(w.stop, 0, sizeof(int32_t), st);
   const int per_tile = token_indices ? 1024 : kTileTokens * K;
   const int n_tiles = token_indices ? route_tiles_general(n_entries) : route_tiles_tc(T);
   if (e == cudaSuccess)

@@ -74,7 +74,8 @@ struct WdArgs {
   __nv_bfloat16* a;  // up output [entries, a_ld], sorted order, permuted columns, zero beyond N / 2
   int a_ld;
   float* y;  // down output [entries, N], sorted order
-  int* err;
+  int* stop;  // 0, or the code of a wait of this call that gave up
+  int* err;   // the caller's error word, which only learns of such a wait
 };
 
 struct WdItem {
@@ -110,9 +111,11 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(p));
   return p != 0;
 }
-// A wait of a whole warp, with one answer for all its lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int where) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, where));
+// A wait of a whole warp, with one answer for all its lanes.  A wait gives up once *stop is set, so that word
+// is this call's own: a routing entry that was rejected, or an error of an earlier call in the caller's word,
+// must not end the waits of a call that is all right.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* stop, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, where));
 }
 
 // Tokens of one of an expert's ceil(n / kN) chunks: equal shares, whole 16s but for the last.
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
           }
           if (ok && j == 0 && h == 0) {  // the MMAs of the stage's last step
             if (step >= kA)
-              ok = warp_wait(&done[half][(step - kA) % kStages], ((step - kA) / kStages) & 1, p.err,
+              ok = warp_wait(&done[half][(step - kA) % kStages], ((step - kA) / kStages) & 1, p.stop,
                              kErrTimeoutProducer);
             tc_fence_after();
           }
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     int li = 0;
     for (int i = blockIdx.x; i < items; i += gridDim.x, ++li) {
       const WdItem it = item_of(i);
-      if (!warp_wait(&tfull, li & 1, p.err, kErrTimeoutEpilogue)) break;
+      if (!warp_wait(&tfull, li & 1, p.stop, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const int pieces = (it.n + 31) / 32;
       for (int piece = 0; piece < 2 * pieces; ++piece) {  // half of the rows, 32 tokens
@@ -369,8 +372,8 @@ __global__ void __launch_bounds__(kWdThreads, 1)
         for (int k = 0; k < p.k_blocks; ++k, ++step) {
           const int s = step % kStages;
           const uint32_t ph = ((step / kStages) & 1) ^ 1;
-          if (!mbar_wait(&done[0][s], ph, p.err, kErrTimeoutProducer) ||
-              !mbar_wait(&done[1][s], ph, p.err, kErrTimeoutProducer)) {
+          if (!mbar_wait(&done[0][s], ph, p.stop, kErrTimeoutProducer) ||
+              !mbar_wait(&done[1][s], ph, p.stop, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -395,13 +398,13 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     for (int i = blockIdx.x; ok && i < items; i += gridDim.x, ++li) {
       const int n = __shfl_sync(0xffffffffu, item_of(i).n, 0);
       const uint32_t idesc = wd_idesc((n + 15) & ~15);
-      if (!warp_wait(&tempty, (li & 1) ^ 1, p.err, kErrTimeoutMma)) break;
+      if (!warp_wait(&tempty, (li & 1) ^ 1, p.stop, kErrTimeoutMma)) break;
       tc_fence_after();
       const uint32_t d = tmem + half * kN;
       for (int k = 0; k < p.k_blocks; ++k, ++step) {
         const int s = step % kStages, g = step % kA;
-        if (!warp_wait(&full_b[s], (step / kStages) & 1, p.err, kErrTimeoutMma) ||
-            !warp_wait(&full_a[half][g], (step / kA) & 1, p.err, kErrTimeoutMma)) {
+        if (!warp_wait(&full_b[s], (step / kStages) & 1, p.stop, kErrTimeoutMma) ||
+            !warp_wait(&full_a[half][g], (step / kA) & 1, p.stop, kErrTimeoutMma)) {
           ok = false;
           break;
         }
@@ -432,6 +435,10 @@ __global__ void __launch_bounds__(kWdThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (tid == 0) {  // a wait that gave up leaves rows unwritten: it outranks a rejected entry
+    const int code = *reinterpret_cast<volatile int*>(p.stop);
+    if (code != 0) atomicExch(p.err, code);
+  }
 }
 
 // Routing plan of few entries (kPlanMaxEntries) and experts (kPlanMaxExperts) in one CTA: counts, offsets,
@@ -445,7 +452,7 @@ template <int kPer>  // entries of a thread
 __global__ void __launch_bounds__(1024)
     wide_plan_kernel(const int32_t* __restrict__ experts, const int32_t* __restrict__ tokens, int n, int T, int K, int E,
                      int32_t* __restrict__ freq, int32_t* __restrict__ off, int32_t* __restrict__ s_rev,
-                     int32_t* __restrict__ x_gather, int32_t* __restrict__ tok_off, int* err, int clear_err) {
+                     int32_t* __restrict__ x_gather, int32_t* __restrict__ tok_off, int* err, int* stop) {
   __shared__ int32_t s_cnt[kPlanMaxExperts], s_sum[32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch();
@@ -453,7 +460,7 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) e[i] = tid + 1024 * i < n ? experts[tid + 1024 * i] : -1;
   s_cnt[tid] = 0;
-  if (clear_err && tid == 0) *err = 0;
+  if (tid == 0) *stop = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -628,9 +635,9 @@ bool int4_plan_fits(int n_entries, int E) { return n_entries <= kPlanMaxEntries 
 
 cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int n, int T, int K, int E, int32_t* freq,
                              int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
-                             bool clear_err, cudaStream_t st) {
+                             int* stop, cudaStream_t st) {
   auto kern = n <= 1024 ? wide_plan_kernel<1> : n <= 4096 ? wide_plan_kernel<4> : wide_plan_kernel<16>;
-  kern<<<1, 1024, 0, st>>>(experts, tokens, n, T, K, E, freq, off, s_rev, x_gather, tok_off, err, clear_err);
+  kern<<<1, 1024, 0, st>>>(experts, tokens, n, T, K, E, freq, off, s_rev, x_gather, tok_off, err, stop);
   return cudaGetLastError();
 }
 
@@ -653,6 +660,7 @@ cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st) {
   u.a = static_cast<__nv_bfloat16*>(p.a);
   u.a_ld = int4_padded(p.I);
   u.y = p.y;
+  u.stop = p.stop;
   u.err = p.err;
   WdArgs d = u;
   d.wq = p.w2q;

@@ -117,16 +117,17 @@ struct Int4Args {
   void* a;   // bf16 [entries, int4_padded(I)] ([entries, I] with few tokens)
   float* y;  // [entries, H]
   void* out;
-  int* err;
+  int* err;   // the caller's error word
+  int* stop;  // launch_int4_wide: zeroed for each call, set by a wait that gives up
 };
 int int4_padded(int K);
 cudaError_t launch_int4_wide(const Int4Args& p, cudaStream_t st);
-// The routing plan of launch_int4_wide in one launch, for sizes that fit; clear_err zeroes *err first.
+// The routing plan of launch_int4_wide in one launch, for sizes that fit; zeroes *stop.
 bool int4_plan_fits(int n_entries, int E);
 cudaError_t launch_int4_plan(const int32_t* experts, const int32_t* tokens, int n, int T, int K, int E, int32_t* freq,
                              int32_t* off, int32_t* s_rev, int32_t* x_gather, int32_t* tok_off, int* err,
-                             bool clear_err, cudaStream_t st);
-// Few tokens: no routing plan (freq is written; off, s_rev, x_gather, tok_off, xs, y unused; err may be null).
+                             int* stop, cudaStream_t st);
+// Few tokens: no routing plan (freq is written; off, s_rev, x_gather, tok_off, xs, y, stop unused; err may be null).
 bool int4_small(const Int4Args& p);
 cudaError_t launch_int4_small(const Int4Args& p, cudaStream_t st);
 
