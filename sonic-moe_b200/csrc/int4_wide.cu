@@ -384,9 +384,10 @@ __global__ void __launch_bounds__(kWdThreads, 1)
                           k * 128 + h * 64, it.base + rows * r, policy);
         }
       }
-      if (!ok)  // let the loads already issued land before shared memory goes away
-        for (int j = max(0, step - kStages); j < step; ++j)
-          mbar_wait_ns(&full_b[j % kStages], (j / kStages) & 1, 50000000ull);
+      // let the loads already issued land before shared memory goes away: an issuer that gave up has not
+      // waited for them
+      for (int j = max(0, step - kStages); j < step; ++j)
+        mbar_wait_ns(&full_b[j % kStages], (j / kStages) & 1, 50000000ull);
     }
   } else {
     // ---------------------------------------------------------------- MMA issuers
