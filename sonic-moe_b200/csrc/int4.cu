@@ -670,13 +670,24 @@ cudaError_t launch_int4_expand(const uint8_t* wq, const void* ws, int E, int N, 
 
 namespace {
 
+// A kernel's limit of dynamic shared memory is one value for all threads of the process: it is set to the most
+// that any call of the instantiation takes, never to one call's own need, which a call beside it could lower
+// before the launch.
+constexpr int kSmMaxExperts = 4096;
+constexpr int kSmResultBytes = 64 * 1024;  // results of a down cluster
+template <int MT, int GPB>
+constexpr int kSmUpBytes = kMvWarps * kDepth * kStage<MT, GPB> + kSmMaxExperts * 4;
+template <int MT, int GPB>
+constexpr int kSmDownBytes = kSmUpBytes<MT, GPB> + kSmResultBytes;
+
 template <int MT, int GPB>
 cudaError_t launch_small_up(SmallArgs p, cudaStream_t st) {
   const int tiles = ceil_div(p.n_tiles, MT);
   const int slots = p.E < p.n_entries ? p.E : p.n_entries;
   auto kern = small_up_kernel<MT, GPB>;
   const int smem = kMvWarps * kDepth * kStage<MT, GPB> + p.E * 4;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > kSmUpBytes<MT, GPB>) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmUpBytes<MT, GPB>);
   if (e != cudaSuccess) return e;
   int occ = 0;
   e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kMvThreads, smem);
@@ -700,11 +711,14 @@ cudaError_t launch_small_down(SmallArgs p, cudaStream_t st) {
   while (cluster < 8 && tiles * cluster < 200 && slots > 8 * cluster) cluster *= 2;
   p.ksplit = 1;
   while (slots * p.ksplit < kMvWarps * cluster && 2 * p.ksplit <= p.k_blocks && p.ksplit < kMvWarps &&
-         2 * p.ksplit * p.n_entries * 64 * MT <= 64 * 1024)
+         2 * p.ksplit * p.n_entries * 64 * MT <= kSmResultBytes)
     p.ksplit *= 2;
   const int smem = kMvWarps * kDepth * kStage<MT, GPB> + p.E * 4 + p.ksplit * p.n_entries * 16 * MT * 4;
+  static_assert(kSmMaxEntries * 64 * MT <= kSmResultBytes && kSmDownBytes<MT, GPB> <= 232448 - 4096,
+                "shared memory budget");
+  if (smem > kSmDownBytes<MT, GPB>) return cudaErrorInvalidValue;
   auto kern = small_down_kernel<MT, GPB>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmDownBytes<MT, GPB>);
   if (e != cudaSuccess) return e;
   return launch_dependent(kern, dim3(tiles * cluster), kMvThreads, smem, cluster, st, p);
 }

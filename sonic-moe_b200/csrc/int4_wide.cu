@@ -604,11 +604,13 @@ __global__ void __launch_bounds__(256)
 
 template <bool kUp, int kN, int GPB>
 cudaError_t launch_wide(const CUtensorMap& t16, const CUtensorMap& t64, const WdArgs& p, int grid, cudaStream_t st) {
-  const int smem = 1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes + (p.E + 1) * 4;
-  static_assert(1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes + 4097 * 4 <= 232448 - 1024,
-                "shared memory budget");
+  constexpr int kFixed = 1024 + WdShape<kN>::kStages * WdShape<kN>::kBStage + WdRing<GPB>::kBytes;
+  constexpr int kMost = kFixed + 4097 * 4;  // set for every call alike: the limit is the whole process's
+  static_assert(kMost <= 232448 - 1024, "shared memory budget");
+  const int smem = kFixed + (p.E + 1) * 4;
+  if (smem > kMost) return cudaErrorInvalidValue;
   auto kern = wide_kernel<kUp, kN, GPB>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
   if (e != cudaSuccess) return e;
   return launch_dependent(kern, dim3(grid), kWdThreads, smem, 1, st, t16, t64, p);
 }
