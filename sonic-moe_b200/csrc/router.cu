@@ -627,9 +627,13 @@ static cudaError_t launch_router_fused_t(const void* x, const void* w, int T, in
     return cudaErrorInvalidValue;
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(E)) cols <<= 1;
-  const int smem = rf_stages(E) * (kRfABytes + E * 128) + (2 * kRfMaxStages + 1) * 8 + 16 + E * 4 + 1024;
+  const auto bytes = [](int experts) {
+    return rf_stages(experts) * (kRfABytes + experts * 128) + (2 * kRfMaxStages + 1) * 8 + 16 + experts * 4 + 1024;
+  };
+  const int smem = bytes(E);
   auto kern = router_fused_kernel<PL, KMAX>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the limit is the whole process's: the same for every call, so that no thread lowers another's
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(256));
   if (e != cudaSuccess) return e;
   kern<<<n_tiles, kRfThreads, smem, st>>>(tx, tw, T, H, E, K, vec, sot, renorm, cols,
                                           static_cast<__nv_bfloat16*>(logits), scores, idx, tile_counts, n_tiles, err);
