@@ -133,15 +133,6 @@ __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint3
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// d = a b + c
-__device__ __forceinline__ void mma_bf16_16816_c(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                 uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
-
 constexpr int kMvWarps = 8;
 constexpr int kMvThreads = 32 * kMvWarps;
 
@@ -158,11 +149,14 @@ constexpr int kMvThreads = 32 * kMvWarps;
 //     weights on the way before it waits for the intermediate.
 // The m16n8k16 tensor core product takes 8 tokens as its 8 columns; with one token 7/8 of its work is
 // thrown away, but it still keeps up with the memory, which the plain FMA units would not beyond 2 tokens.
-// What bounds it: integer instructions, which an SM issues at half rate.  Turning 2048 codes into bf16 takes
-// a warp 56 of them (28 cycles of an SM) and some 25 for the ring, against 44 cycles that their bytes take
-// at the HBM rate; with the latencies in between the layer streams at 3.3 TB/s (8 tokens, 4096 x 1024, 128
-// experts: 107 us; one token 28.6 us).  Registers instead of the shared-memory ring, a block of x without the
-// read-ahead, and 1 or 4 row tiles a warp all measured slower.
+// What it spends its time on: turning 2048 codes into bf16 takes a warp 56 integer instructions, which an SM
+// issues at half rate (28 cycles of it), 32 packed bf16 ones and some 25 for the ring, against 44 cycles that
+// their bytes take at the HBM rate.  Neither unit is full: at 8 tokens of 4096 x 1024 (64 experts) the up kernel
+// issues in 60% of the cycles with its integer pipe at 57% and DRAM at 35%, the down kernel in 44% (40%, 25%);
+// the rest is latency.  8 tokens of 4096 x 1024 with 128 experts take 103 us, one token 26 us.  Scaling the
+// groups' sums instead of the weights is up to 5% faster (groups of 64: 102 us against 106) but wrong for large
+// x, see use_stage.  Registers instead of the shared-memory ring, and a block of x without the read-ahead,
+// measured slower.
 
 constexpr int kSmMaxEntries = 256;  // their down results are kept in shared memory (128 bytes an entry)
 
@@ -341,17 +335,16 @@ __device__ __forceinline__ void load_x(uint4 (&x)[4], const __nv_bfloat16* xrow,
   }
 }
 
-// One stage's products.  The instructions per weight count here: a group's sums are scaled, in fp32, and
-// the offset of the codes (16 + n stands for q + 24) is taken from the sums too, which start at -24 times
-// the sum of x, itself a product with a constant.
+// One stage's products.  The weights enter them with their scale, as exact bf16 numbers: taking the codes' offset
+// from a sum of (16 + n) x afterwards would leave an error of 24 |x| in it, whatever the code, and overflow where
+// the sum itself does not.
 template <int MT, int GPB>
 __device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage, const uint4 (&x)[4],
                                           float (&acc)[MT][4]) {
-  constexpr uint32_t kMinus24 = 0xC1C0C1C0u;
   const int lane = threadIdx.x & 31;
-  float part[MT][4], c[4];
   uint4 q[MT];
   uint32_t s2[MT][GPB];
+  __nv_bfloat162 sl[MT], sh[MT], ml[MT], mh[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const uint32_t a = stage + 1024 * MT + 128 * GPB * m + 4 * GPB * lane;
@@ -368,41 +361,25 @@ __device__ __forceinline__ void use_stage(const Int4Magic& magic, uint32_t stage
   }
 #pragma unroll
   for (int s = 0; s < 4; ++s) {  // 32 columns each
-    const bool first = s % (4 / GPB) == 0, last = (s + 1) % (4 / GPB) == 0;
-    if (first) {
-#pragma unroll
-      for (int i = s; i < s + 4 / GPB; ++i) {
-        if (i == s)
-          mma_bf16_16816_c(c, kMinus24, kMinus24, kMinus24, kMinus24, x[i].x, x[i].y, 0.0f, 0.0f, 0.0f, 0.0f);
-        else
-          mma_bf16_16816(c, kMinus24, kMinus24, kMinus24, kMinus24, x[i].x, x[i].y);
-        mma_bf16_16816(c, kMinus24, kMinus24, kMinus24, kMinus24, x[i].z, x[i].w);
-      }
-    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      if (s % (4 / GPB) == 0) {  // a group's first columns
+        const uint32_t w = s2[m][s / (4 / GPB)];
+        sl[m] = int4_scale2(w, 0);
+        sh[m] = int4_scale2(w, 1);
+        ml[m] = int4_m24(sl[m]);
+        mh[m] = int4_m24(sh[m]);
+      }
       if (s % 2 == 0) q[m] = lds128(stage + 1024 * m + 256 * s + 16 * lane);
       const uint32_t wl = s & 1 ? q[m].z : q[m].x, wh = s & 1 ? q[m].w : q[m].y;
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        lo[i] = int4_raw(magic, wl, i);
-        hi[i] = int4_raw(magic, wh, i);
+        lo[i] = int4_scaled(magic, wl, i, sl[m], ml[m]);
+        hi[i] = int4_scaled(magic, wh, i, sh[m], mh[m]);
       }
-      float(&d)[4] = part[m];
-      if (first)
-        mma_bf16_16816_c(d, lo[0], hi[0], lo[1], hi[1], x[s].x, x[s].y, c[0], c[1], c[2], c[3]);
-      else
-        mma_bf16_16816(d, lo[0], hi[0], lo[1], hi[1], x[s].x, x[s].y);
-      mma_bf16_16816(d, lo[2], hi[2], lo[3], hi[3], x[s].z, x[s].w);
-      if (last) {
-        const uint32_t w = s2[m][s / (4 / GPB)];
-        const float slo = __uint_as_float(w << 16), shi = __uint_as_float(w & 0xFFFF0000u);
-        acc[m][0] = fmaf(slo, d[0], acc[m][0]);
-        acc[m][1] = fmaf(slo, d[1], acc[m][1]);
-        acc[m][2] = fmaf(shi, d[2], acc[m][2]);
-        acc[m][3] = fmaf(shi, d[3], acc[m][3]);
-      }
+      mma_bf16_16816(acc[m], lo[0], hi[0], lo[1], hi[1], x[s].x, x[s].y);
+      mma_bf16_16816(acc[m], lo[2], hi[2], lo[3], hi[3], x[s].z, x[s].w);
     }
   }
 }
@@ -736,17 +713,19 @@ cudaError_t launch_small(const SmallArgs& u, int group1, const SmallArgs& d, int
 
 }  // namespace
 
-// Row tiles of a warp's item: 2 (8 tokens, 4096 x 1024: 107 us; 1: 140 us, 4: 118 us).
+// Row tiles of a warp's item (4096 x 1024, 128 experts, groups of 128, us with 1 / 2 / 4): one token 23 / 26 / 28,
+// 2 tokens 39 / 36 / 55, 4 tokens 70 / 61 / 70, 8 tokens 109 / 105 / 128.
 constexpr int kMT = 2;
 
 // Up to 8 tokens an expert's tokens fit the 8 columns of a product and nothing is read twice; beyond, that
-// depends on the routing (4096 x 1024, 128 experts, us, this / the other: 16 tokens even 142 / 162, Zipf 115 /
-// 109; 24 tokens 180 / 193 and 180 / 135).  With groups of 64 or 128 this path is then the faster one but for
-// single points (1, 4 and 8 tokens of 4096 x 1024 29 / 40, 63 / 78, 112 / 116; 4 and 8 of 2048 x 768 34 / 45,
-// 52 / 60; 1, 4 and 8 of 7168 x 2048 with 64 experts 58 / 70, 185 / 168, 238 / 254).  Groups of 32 cost its
-// warps more, since every group's sum is scaled apart: the other path wins from about 2 10^8 weights a matrix
-// on (4096 x 1024 at 6 and 8 tokens, 2.0 and 2.7 10^8: 100 / 102, 128 / 116; 7168 x 2048 at 2 and 4, 2.3 and
-// 4.7 10^8: 118 / 115, 210 / 167).
+// depends on the routing (before its weights were scaled ahead of the products, 4096 x 1024, 128 experts, us, this /
+// the other: 16 tokens even 142 / 162, Zipf 115 / 109; 24 tokens 180 / 193 and 180 / 135).  With groups of 64 or
+// 128 this path is then the faster one or within 8% of it (us, this / the other, groups of 128: 1, 4 and 8 tokens
+// of 4096 x 1024 26 / 38, 61 / 75, 103 / 105; of 2048 x 768 16 / 27, 32 / 43, 48 / 56; of 7168 x 2048 with 64
+// experts 56 / 67, 189 / 189, 272 / 269; groups of 64: 64 / 73 and 107 / 103 at 4 and 8 tokens of 4096 x 1024,
+// 200 / 185 and 295 / 281 of 7168 x 2048).  Groups of 32 cost its warps more scales: the other path wins from about
+// 2 10^8 weights a matrix on (4096 x 1024 at 4, 6 and 8 tokens, 1.3, 2.0 and 2.7 10^8: 72 / 76, 98 / 97, 119 / 106;
+// 7168 x 2048 at 1, 2 and 4, 1.2, 2.3 and 4.7 10^8: 66 / 67, 118 / 114, 222 / 202).
 bool int4_small(const Int4Args& p) {
   if (p.T > 8 || p.n_entries > kSmMaxEntries) return false;
   const size_t weights = static_cast<size_t>(p.n_entries < p.E ? p.n_entries : p.E) * p.H * p.I;
