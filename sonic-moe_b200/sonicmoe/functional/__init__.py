@@ -41,6 +41,7 @@ gradient is requested, instead of returning an output whose weights would never 
 import weakref
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 from .. import ops
@@ -489,33 +490,81 @@ def moe_general_routing_inputs(
     return _fp8_moe_general_forward(*args, w1, w2, concat_layout)
 
 
+def _has_tangent(t) -> bool:
+    return fwAD.unpack_dual(t).tangent is not None
+
+
+def _switch_loss_gradient(router_logits, coef, token_mask):
+    """dloss/dlogits [T, E] fp32 in torch operations, which any transform can follow."""
+    z, on = router_logits, None
+    if token_mask is not None:  # what a left-out row holds must not reach a second gradient either
+        on = token_mask[:, None] != 0
+        z = z.where(on, 0.0)
+    p = F.softmax(z, dim=-1, dtype=torch.float32)
+    if on is not None:
+        p = p.where(on, 0.0)
+    return p * (coef - (p * coef).sum(-1, keepdim=True))
+
+
 class _SwitchLossFunction(torch.autograd.Function):
-    """Balance loss with its gradient for the router logits; the counts carry none."""
+    """Balance loss with its derivatives for the router logits; the counts carry none."""
 
     @staticmethod
     def forward(ctx, router_logits, expert_frequency, topk_indices, token_mask):
         loss, freq, coef = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
         ctx.save_for_backward(router_logits, coef, token_mask)
+        ctx.save_for_forward(router_logits, coef, token_mask)
         ctx.mark_non_differentiable(freq)
         ctx.set_materialize_grads(False)
         return loss, freq
 
     @staticmethod
-    def backward(ctx, dloss, _dfreq):
+    def backward(ctx, dloss, *_):
         if dloss is None:
             return None, None, None, None
         router_logits, coef, token_mask = ctx.saved_tensors
-        if torch.is_grad_enabled():  # create_graph: the same formula in operations autograd can follow
-            z, on = router_logits, None
-            if token_mask is not None:  # what a left-out row holds must not reach the second gradient either
-                on = token_mask[:, None] != 0
-                z = z.where(on, 0.0)
-            p = F.softmax(z, dim=-1, dtype=torch.float32)
-            if on is not None:
-                p = p.where(on, 0.0)
-            dl = dloss * p * (coef - (p * coef).sum(-1, keepdim=True))
+        # create_graph, a transform around this, a batch of gradients (which has no storage to point to) or forward
+        # mode through the backward: the same formula in operations that can be followed
+        if (torch.is_grad_enabled() or torch._C._are_functorch_transforms_active()
+                or torch._C._functorch.is_legacy_batchedtensor(dloss) or _has_tangent(router_logits)
+                or _has_tangent(dloss)):
+            dl = dloss * _switch_loss_gradient(router_logits, coef, token_mask)
             return dl.to(router_logits.dtype), None, None, None
         return ops.switch_loss_bwd(router_logits, coef, dloss.to(torch.float32), token_mask), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        if tangent is None:
+            return None, None
+        return (_switch_loss_gradient(*ctx.saved_tensors) * tangent).sum(), None
+
+
+class _SwitchLossTransformed(_SwitchLossFunction):
+    """The same for torch.func's transforms, which need the context set up apart and a rule for batches.  (Apart,
+    since such a function costs an eager call 30 us more.)"""
+
+    @staticmethod
+    def forward(router_logits, expert_frequency, topk_indices, token_mask):
+        return ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        router_logits, _, _, token_mask = inputs
+        _, freq, coef = output
+        ctx.save_for_backward(router_logits, coef, token_mask)
+        ctx.save_for_forward(router_logits, coef, token_mask)
+        ctx.mark_non_differentiable(freq, coef)
+        ctx.set_materialize_grads(False)
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        return *_SwitchLossFunction.jvp(ctx, tangent), None
+
+    @staticmethod
+    def vmap(info, in_dims, *args):
+        outs = [_SwitchLossTransformed.apply(*(a if d is None else a.select(d, i).contiguous()
+                                               for a, d in zip(args, in_dims))) for i in range(info.batch_size)]
+        return tuple(torch.stack(o) for o in zip(*outs)), (0, 0, 0)
 
 
 @torch.library.custom_op("sonicmoe::switch_loss", mutates_args=())
@@ -566,7 +615,8 @@ def switch_load_balancing_loss(
     token_mask: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Switch load-balancing loss of the router (the formula of reference moe.py:263-276) and the experts'
-    counts: (loss fp32 [], expert_frequency int32 [E]), differentiable with respect to router_logits.
+    counts: (loss fp32 [], expert_frequency int32 [E]), differentiable with respect to router_logits (backward,
+    forward mode, torch.func's transforms, and any of them again).
 
         p = softmax(router_logits), loss = E * sum_e (sum_t p[t, e] / sum p) (f_e / sum f)
 
@@ -589,10 +639,12 @@ def switch_load_balancing_loss(
         token_mask = token_mask.contiguous()
     if torch.compiler.is_compiling():
         loss, freq, _ = _switch_loss_op(router_logits, expert_frequency, topk_indices, token_mask)
-    elif not (router_logits.requires_grad and torch.is_grad_enabled()):
-        loss, freq, _ = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
-    else:
+    elif torch._C._are_functorch_transforms_active():
+        loss, freq, _ = _SwitchLossTransformed.apply(router_logits, expert_frequency, topk_indices, token_mask)
+    elif router_logits.requires_grad and torch.is_grad_enabled() or _has_tangent(router_logits):
         loss, freq = _SwitchLossFunction.apply(router_logits, expert_frequency, topk_indices, token_mask)
+    else:
+        loss, freq, _ = ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
     return loss, freq
 
 
