@@ -485,6 +485,15 @@ int sm_switch_loss(const void* router_logits, int dtype, int T, int E, const uin
                    const int32_t* topk_indices, int K, const int32_t* expert_frequency, float* loss, float* coef,
                    int32_t* expert_frequency_out, void* workspace, size_t workspace_bytes, int32_t* err,
                    void* stream);
+/* The same with the counts as given in another type: int64, or float32 / float64 for fractions of the entries and
+ * averages of counts (no count below 0).  Only their proportions matter. */
+#define SM_COUNT_I32 0
+#define SM_COUNT_I64 1
+#define SM_COUNT_F32 2
+#define SM_COUNT_F64 3
+int sm_switch_loss_counts(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                          const void* counts, int count_type, float* loss, float* coef, void* workspace,
+                          size_t workspace_bytes, void* stream);
 /* dlogits [T, E] (the logits' dtype) = *dloss * dloss/dlogits; rows of tokens that do not count are 0. */
 int sm_switch_loss_bwd(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
                        const float* coef, const float* dloss, void* dlogits, void* stream);

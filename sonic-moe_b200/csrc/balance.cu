@@ -6,8 +6,8 @@
 //   dloss/dlogits[t, e] = p[t, e] (c_e - sum_j p[t, j] c_j),   c_e = (E f_e - F) / (F n)
 //
 // (sum_e p[t, e] = 1, so neither the normalisation of P by n nor a constant added to c changes the
-// gradient; taking E f_e - F in integers instead of E f_e keeps c free of the cancellation that a
-// nearly balanced routing would otherwise bring.)
+// gradient; taking E f_e - F in 64 bits, where whole counts are exact, instead of E f_e keeps c free of the
+// cancellation that a nearly balanced routing would otherwise bring.)
 //
 // switch_loss_kernel        one pass over the logits: softmax of each row in registers, its columns
 //                           summed per thread, over the CTA and over a cluster of 8 CTAs; counts of the
@@ -232,12 +232,30 @@ __device__ __forceinline__ uint32_t ld_cluster(const void* p, int rank) {
   return v;
 }
 
+// Counts as given: whole numbers, or fractions and averages of counts.
+struct Counts {
+  const void* p;
+  int type;  // CountType
+  __device__ __forceinline__ double at(int e) const {
+    switch (type) {
+      case kCountI32:
+        return static_cast<const int32_t*>(p)[e];
+      case kCountI64:
+        return static_cast<double>(static_cast<const long long*>(p)[e]);
+      case kCountF32:
+        return static_cast<const float*>(p)[e];
+      default:
+        return static_cast<const double*>(p)[e];
+    }
+  }
+};
+
 // The threads' x and f summed over the CTA, in a fixed order; every thread gets the sums.
 struct FinishSums {
   float x[32];
-  long long f[32];
+  double f[32];
 };
-__device__ __forceinline__ void block_sums(float& x, long long& f, FinishSums& sm) {
+__device__ __forceinline__ void block_sums(float& x, double& f, FinishSums& sm) {
   __syncthreads();
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) {
@@ -250,54 +268,56 @@ __device__ __forceinline__ void block_sums(float& x, long long& f, FinishSums& s
   }
   __syncthreads();
   x = 0.0f;
-  f = 0;
+  f = 0.0;
   for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
     x += sm.x[w];
     f += sm.f[w];
   }
 }
 
-// P (column sums) and f (counts) of the CTA's experts e0 .. e0 + n_own - 1 in shared memory -> loss, c,
-// counts.  kClustered: the CTAs of a cluster hold the experts between them.
+// P (column sums) and f (counts) of the CTA's experts e0 .. e0 + n_own - 1 -> loss, c, counts; s_p and, unless it
+// is null, s_f lie in shared memory, other counts are those given.  kClustered: the CTAs of a cluster hold the
+// experts between them.
 template <bool kClustered>
-__device__ void finish(const float* s_p, const int32_t* s_f, int E, int e0, int n_own, float* __restrict__ loss,
-                       float* __restrict__ coef, int32_t* __restrict__ freq_out) {
+__device__ void finish(const float* s_p, const int32_t* s_f, const Counts& given, int E, int e0, int n_own,
+                       float* __restrict__ loss, float* __restrict__ coef, int32_t* __restrict__ freq_out) {
   __shared__ FinishSums s_sums;
   __shared__ float s_x[2];  // the CTA's sum of P, its part of the loss
-  __shared__ int32_t s_count[2];
+  __shared__ double s_count;  // its sum of f
+  auto count = [&](int e) { return s_f ? static_cast<double>(s_f[e]) : given.at(e0 + e); };
   float n = 0.0f;
-  long long F = 0;
+  double F = 0.0;
   for (int e = threadIdx.x; e < n_own; e += blockDim.x) {
     n += s_p[e];
-    F += s_f[e];
+    F += count(e);
   }
   block_sums(n, F, s_sums);
   if constexpr (kClustered) {
     if (threadIdx.x == 0) {
       s_x[0] = n;
-      s_count[0] = static_cast<int32_t>(F & 0xffffffff);
-      s_count[1] = static_cast<int32_t>(F >> 32);
+      s_count = F;
     }
     cluster_sync();
     n = 0.0f;
-    F = 0;
+    F = 0.0;
 #pragma unroll
     for (int k = 0; k < kSlCluster; ++k) {
       n += __uint_as_float(ld_cluster(&s_x[0], k));
-      F += static_cast<long long>(static_cast<unsigned long long>(ld_cluster(&s_count[1], k)) << 32 |
-                                  ld_cluster(&s_count[0], k));
+      const uint32_t* half = reinterpret_cast<const uint32_t*>(&s_count);
+      F += __hiloint2double(ld_cluster(half + 1, k), ld_cluster(half, k));
     }
   }
   // no token counts, or no entry: the loss and the gradient are 0 (a NaN sum stays NaN)
   const float inv_n = n == 0.0f ? 0.0f : 1.0f / n;
-  const float inv_f = F == 0 ? 0.0f : 1.0f / static_cast<float>(F);
+  const float inv_f = F == 0.0 ? 0.0f : 1.0f / static_cast<float>(F);
   float l = 0.0f;
   for (int e = threadIdx.x; e < n_own; e += blockDim.x) {
-    l += (s_p[e] * inv_n) * (static_cast<float>(s_f[e]) * inv_f);
-    coef[e0 + e] = static_cast<float>(static_cast<long long>(s_f[e]) * E - F) * inv_f * inv_n;
-    if (freq_out) freq_out[e0 + e] = s_f[e];
+    const double f = count(e);
+    l += (s_p[e] * inv_n) * (static_cast<float>(f) * inv_f);
+    coef[e0 + e] = static_cast<float>(f * E - F) * inv_f * inv_n;
+    if (freq_out) freq_out[e0 + e] = static_cast<int32_t>(f);
   }
-  long long none = 0;
+  double none = 0.0;
   block_sums(l, none, s_sums);
   if constexpr (kClustered) {
     if (threadIdx.x == 0) s_x[1] = l;
@@ -318,9 +338,8 @@ __device__ void finish(const float* s_p, const int32_t* s_f, int E, int e0, int 
 template <typename InT, int L, int C>
 __global__ void __launch_bounds__(kSlThreads)
     switch_loss_kernel(const InT* __restrict__ logits, int T, int E, int vec, const uint8_t* __restrict__ mask,
-                       const int32_t* __restrict__ idx, int K, const int32_t* __restrict__ freq_in,
-                       float* __restrict__ part_p, int32_t* __restrict__ part_f, float* __restrict__ loss,
-                       float* __restrict__ coef, int32_t* __restrict__ freq_out, int* __restrict__ err) {
+                       const int32_t* __restrict__ idx, int K, const Counts given, float* __restrict__ part_p,
+                       int32_t* __restrict__ part_f, float* __restrict__ loss, float* __restrict__ coef, int32_t* __restrict__ freq_out, int* __restrict__ err) {
   constexpr int kGroups = kSlThreads / L;               // rows of a CTA's step
   constexpr int kCopies = L < 32 ? kSlThreads / 32 : kGroups;
   extern __shared__ float s_dyn[];
@@ -410,11 +429,10 @@ __global__ void __launch_bounds__(kSlThreads)
     float p = s_p[e];
     for (int k = 1; k < kCopies; ++k) p += s_p[static_cast<size_t>(k) * E + e];
     s_p[e] = p;
-    if (gridDim.x == 1 && !idx) s_f[e] = freq_in[e];
   }
   if (gridDim.x == 1) {
     __syncthreads();
-    finish<false>(s_p, s_f, E, 0, E, loss, coef, freq_out);
+    finish<false>(s_p, idx ? s_f : nullptr, given, E, 0, E, loss, coef, freq_out);
     return;
   }
   // the cluster's CTAs each add an eighth of the columns over all 8
@@ -445,8 +463,8 @@ constexpr int kFinOneCta = 256;
 template <bool kClustered>
 __global__ void __launch_bounds__(kFinThreads)
     switch_loss_finish_kernel(const float* __restrict__ part_p, const int32_t* __restrict__ part_f, int parts, int E,
-                              int slices, const int32_t* __restrict__ freq_in, float* __restrict__ loss,
-                              float* __restrict__ coef, int32_t* __restrict__ freq_out) {
+                              int slices, const Counts given, float* __restrict__ loss, float* __restrict__ coef,
+                              int32_t* __restrict__ freq_out) {
   __shared__ float s_p[kFinThreads];
   __shared__ int32_t s_f[kFinThreads];
   const int own = kClustered ? (E + kSlCluster - 1) / kSlCluster : E;  // slices * own <= kFinThreads
@@ -473,10 +491,10 @@ __global__ void __launch_bounds__(kFinThreads)
       f += s_f[k * own + threadIdx.x];
     }
     s_p[threadIdx.x] = p;
-    s_f[threadIdx.x] = part_f ? f : freq_in[e0 + threadIdx.x];
+    s_f[threadIdx.x] = f;
   }
   __syncthreads();
-  finish<kClustered>(s_p, s_f, E, e0, n_own, loss, coef, freq_out);
+  finish<kClustered>(s_p, part_f ? s_f : nullptr, given, E, e0, n_own, loss, coef, freq_out);
 }
 
 template <typename InT, int L, int C>
@@ -566,7 +584,7 @@ struct SlArgs {
   const uint8_t* mask;
   const int32_t* idx;
   int K;
-  const int32_t* freq_in;
+  Counts given;
   float* part_p;
   int32_t* part_f;
   float* loss;
@@ -595,7 +613,7 @@ cudaError_t launch_lc(const SlArgs& a, bool bwd, cudaStream_t st) {
   const int vec = vec_of(a.logits, a.E, sizeof(InT));
   cudaError_t e;
   if (a.grid == 1) {
-    kern<<<1, kSlThreads, smem, st>>>(x, a.T, a.E, vec, a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss, a.coef,
+    kern<<<1, kSlThreads, smem, st>>>(x, a.T, a.E, vec, a.mask, a.idx, a.K, a.given, a.part_p, a.part_f, a.loss, a.coef,
                                       a.freq_out, a.err);
     return cudaGetLastError();
   }
@@ -611,14 +629,14 @@ cudaError_t launch_lc(const SlArgs& a, bool bwd, cudaStream_t st) {
   at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, x, a.T, a.E, vec, a.mask, a.idx, a.K, a.freq_in, a.part_p, a.part_f, a.loss, a.coef,
+  e = cudaLaunchKernelEx(&cfg, kern, x, a.T, a.E, vec, a.mask, a.idx, a.K, a.given, a.part_p, a.part_f, a.loss, a.coef,
                          a.freq_out, a.err);
   if (e != cudaSuccess) return e;
   const bool one = a.E <= kFinOneCta;
   const int ctas = one ? 1 : kSlCluster, slices = kFinThreads / ceil_div(a.E, ctas);
   return launch_dependent(one ? switch_loss_finish_kernel<false> : switch_loss_finish_kernel<true>, dim3(ctas),
                           kFinThreads, 0, ctas, st, a.part_p, a.idx ? a.part_f : nullptr, a.grid, a.E,
-                          slices < 32 ? slices : 32, a.freq_in, a.loss, a.coef, a.freq_out);
+                          slices < 32 ? slices : 32, a.given, a.loss, a.coef, a.freq_out);
 }
 
 // Lanes per row: as many as hold the row at 8 values each, up to a warp; wider rows take 16 or 32
@@ -657,9 +675,9 @@ int switch_loss_parts(int T, int E) {
 }
 
 cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,
-                               int K, const int32_t* freq_in, float* part_p, int32_t* part_f, float* loss,
+                               int K, const void* counts, int count_type, float* part_p, int32_t* part_f, float* loss,
                                float* coef, int32_t* freq_out, int* err, cudaStream_t st) {
-  SlArgs a{logits, T, E, mask, idx, K, freq_in, part_p, part_f, loss, coef, freq_out, err, nullptr, nullptr,
+  SlArgs a{logits, T, E, mask, idx, K, Counts{counts, count_type}, part_p, part_f, loss, coef, freq_out, err, nullptr, nullptr,
            switch_loss_parts(T, E)};
   return launch(a, dtype, false, st);
 }

@@ -814,9 +814,24 @@ int sm_switch_loss(const void* router_logits, int dtype, int T, int E, const uin
   SlWs w = carve_switch_loss(c, T, E);
   if (!c.ok) return fail(SM_EINVAL, "workspace too small (%zu < %zu)", workspace_bytes, c.used);
   return cuda_status(launch_switch_loss(router_logits, dtype, T, E, token_mask, topk_indices, K, expert_frequency,
-                                        w.part_p, w.part_f, loss, coef, expert_frequency_out, err ? err : w.err,
+                                        kCountI32, w.part_p, w.part_f, loss, coef, expert_frequency_out, err ? err : w.err,
                                         static_cast<cudaStream_t>(stream)),
                      "switch_loss");
+}
+
+int sm_switch_loss_counts(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,
+                          const void* counts, int count_type, float* loss, float* coef, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  int rc = check_switch_loss_args(T, E, dtype);
+  if (rc) return rc;
+  if (count_type < SM_COUNT_I32 || count_type > SM_COUNT_F64) return fail(SM_EINVAL, "unknown count type %d", count_type);
+  if ((T > 0 && !router_logits) || !counts || !loss || !coef || !workspace) return fail(SM_EINVAL, "null pointer");
+  Carve c{static_cast<uint8_t*>(workspace), workspace_bytes};
+  SlWs w = carve_switch_loss(c, T, E);
+  if (!c.ok) return fail(SM_EINVAL, "workspace too small (%zu < %zu)", workspace_bytes, c.used);
+  return cuda_status(launch_switch_loss(router_logits, dtype, T, E, token_mask, nullptr, 0, counts, count_type, w.part_p,
+                                        w.part_f, loss, coef, nullptr, w.err, static_cast<cudaStream_t>(stream)),
+                     "switch_loss_counts");
 }
 
 int sm_switch_loss_bwd(const void* router_logits, int dtype, int T, int E, const uint8_t* token_mask,

@@ -80,9 +80,10 @@ cudaError_t launch_router_bwd(const void* logits, const float* scores, const int
                               int E, int K, int sot, int renorm, float* dlogits, cudaStream_t st);
 
 // router balance loss (csrc/balance.cu); parts = rows of the partial sums part_p / part_f [parts, E]
+enum CountType { kCountI32 = 0, kCountI64 = 1, kCountF32 = 2, kCountF64 = 3 };
 int switch_loss_parts(int T, int E);
 cudaError_t launch_switch_loss(const void* logits, int dtype, int T, int E, const uint8_t* mask, const int32_t* idx,
-                               int K, const int32_t* freq_in, float* part_p, int32_t* part_f, float* loss,
+                               int K, const void* counts, int count_type, float* part_p, int32_t* part_f, float* loss,
                                float* coef, int32_t* freq_out, int* err, cudaStream_t st);
 cudaError_t launch_switch_loss_bwd(const void* logits, int dtype, int T, int E, const uint8_t* mask,
                                    const float* coef, const float* dloss, void* dlogits, cudaStream_t st);

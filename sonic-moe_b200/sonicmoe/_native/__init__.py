@@ -120,6 +120,7 @@ SIGNATURES = {
     ),
     "sm_switch_loss_workspace": (_SZ, [_I, _I]),
     "sm_switch_loss": (_I, [_P, _I, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _SZ, _P, _P]),
+    "sm_switch_loss_counts": (_I, [_P, _I, _I, _I, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "sm_switch_loss_bwd": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
     "sm_int4_weight_bytes": (_SZ, [_I, _I, _I]),
     "sm_int4_scale_count": (_SZ, [_I, _I, _I, _I]),

@@ -491,7 +491,7 @@ def moe_general_routing_inputs(
 
 
 def _has_tangent(t) -> bool:
-    return fwAD.unpack_dual(t).tangent is not None
+    return fwAD._current_level >= 0 and fwAD.unpack_dual(t).tangent is not None
 
 
 def _switch_loss_gradient(router_logits, coef, token_mask):
@@ -533,7 +533,9 @@ class _SwitchLossFunction(torch.autograd.Function):
         return ops.switch_loss_bwd(router_logits, coef, dloss.to(torch.float32), token_mask), None, None, None
 
     @staticmethod
-    def jvp(ctx, tangent, *_):
+    def jvp(ctx, tangent, counts_tangent, *_):
+        if counts_tangent is not None:
+            raise NotImplementedError("expert_frequency carries no derivative; give it without a tangent")
         if tangent is None:
             return None, None
         return (_switch_loss_gradient(*ctx.saved_tensors) * tangent).sum(), None
@@ -557,8 +559,8 @@ class _SwitchLossTransformed(_SwitchLossFunction):
         ctx.set_materialize_grads(False)
 
     @staticmethod
-    def jvp(ctx, tangent, *_):
-        return *_SwitchLossFunction.jvp(ctx, tangent), None
+    def jvp(ctx, *tangents):
+        return *_SwitchLossFunction.jvp(ctx, *tangents), None
 
     @staticmethod
     def vmap(info, in_dims, *args):
@@ -574,14 +576,15 @@ def _switch_loss_op(
     topk_indices: torch.Tensor | None,
     token_mask: torch.Tensor | None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """``ops.switch_loss`` for traced callers: (loss fp32 [], counts int32 [E], coef fp32 [E])."""
+    """``ops.switch_loss`` for traced callers: (loss fp32 [], counts [E], coef fp32 [E])."""
     return ops.switch_loss(router_logits, expert_frequency, topk_indices, token_mask)
 
 
 @_switch_loss_op.register_fake
 def _(router_logits, expert_frequency, topk_indices, token_mask):
     E = router_logits.shape[1]
-    return (router_logits.new_empty((), dtype=torch.float32), router_logits.new_empty(E, dtype=torch.int32),
+    counts = torch.int32 if expert_frequency is None else expert_frequency.dtype
+    return (router_logits.new_empty((), dtype=torch.float32), router_logits.new_empty(E, dtype=counts),
             router_logits.new_empty(E, dtype=torch.float32))
 
 
@@ -608,6 +611,23 @@ def _switch_loss_backward(ctx, dloss, _dfreq, _dcoef):
 _switch_loss_op.register_autograd(_switch_loss_backward, setup_context=_switch_loss_setup)
 
 
+# exact conversions of given counts to a type the kernels read
+_COUNT_AS = {torch.bool: torch.int32, torch.uint8: torch.int32, torch.int8: torch.int32, torch.int16: torch.int32,
+             torch.float16: torch.float32, torch.bfloat16: torch.float32}
+
+
+def _given_counts(expert_frequency):
+    if expert_frequency.dtype is torch.int32:
+        return expert_frequency.contiguous()
+    if expert_frequency.is_floating_point():
+        if expert_frequency.requires_grad and torch.is_grad_enabled() or _has_tangent(expert_frequency):
+            raise ValueError("expert_frequency gets no gradient; give it detached")
+    dtype = _COUNT_AS.get(expert_frequency.dtype, expert_frequency.dtype)
+    if dtype not in ops._COUNT_TYPES:
+        raise ValueError(f"expert_frequency must hold whole or real numbers, got {expert_frequency.dtype}")
+    return expert_frequency.to(dtype).contiguous()
+
+
 def switch_load_balancing_loss(
     router_logits: torch.Tensor,
     expert_frequency: torch.Tensor | None = None,
@@ -615,15 +635,16 @@ def switch_load_balancing_loss(
     token_mask: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Switch load-balancing loss of the router (the formula of reference moe.py:263-276) and the experts'
-    counts: (loss fp32 [], expert_frequency int32 [E]), differentiable with respect to router_logits (backward,
+    counts: (loss fp32 [], expert_frequency [E]), differentiable with respect to router_logits (backward,
     forward mode, torch.func's transforms, and any of them again).
 
         p = softmax(router_logits), loss = E * sum_e (sum_t p[t, e] / sum p) (f_e / sum f)
 
     Args:
         router_logits: [T, E], bf16, fp16 or fp32.
-        expert_frequency: [E] counts f, as ``moe_TC_softmax_topk_layer`` returns them; or
-        topk_indices: [T, K] expert ids, as ``ops.router_topk`` returns them, which are counted here.
+        expert_frequency: [E] counts f, as ``moe_TC_softmax_topk_layer`` returns them, or any numbers >= 0
+            in their proportions (fractions of the entries, counts averaged over ranks); or
+        topk_indices: [T, K] expert ids, as ``ops.router_topk`` returns them, which are counted here in int32.
             Exactly one of the two is given; neither gets a gradient.
         token_mask: [T] bool, optional: tokens that are False (padding) take no part in the
             probabilities, in the counts made from topk_indices, or in the gradient.
@@ -632,7 +653,7 @@ def switch_load_balancing_loss(
     """
     router_logits = router_logits.contiguous()
     if expert_frequency is not None:
-        expert_frequency = expert_frequency.to(torch.int32).contiguous()
+        expert_frequency = _given_counts(expert_frequency)
     if topk_indices is not None:
         topk_indices = topk_indices.to(torch.int32).contiguous()
     if token_mask is not None:

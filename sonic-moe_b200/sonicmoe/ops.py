@@ -628,13 +628,17 @@ def _check_logits(router_logits: torch.Tensor):
         raise ValueError(f"unsupported logits dtype {router_logits.dtype}")
 
 
+# types of given counts (SM_COUNT_*)
+_COUNT_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
 def switch_loss(router_logits: torch.Tensor, expert_frequency: torch.Tensor = None, topk_indices: torch.Tensor = None,
                 token_mask: torch.Tensor = None, err: torch.Tensor = None):
     """Switch balance loss of the router (reference moe.py:263-276) and the counts it used: (loss fp32 [],
-    expert_frequency int32 [E], coef fp32 [E] for ``switch_loss_bwd``).
+    expert_frequency [E], coef fp32 [E] for ``switch_loss_bwd``).
 
-    router_logits [T, E]; exactly one of expert_frequency (int32 [E], counts as given) and topk_indices
-    (int32 [T, K], counted here).  token_mask [T] (bool or uint8): tokens with 0, such as padding, count
+    router_logits [T, E]; exactly one of expert_frequency ([E] int32, int64, fp32 or fp64: counts as given, a copy of
+    which comes back) and topk_indices (int32 [T, K], counted here in int32).  token_mask [T] (bool or uint8): tokens with 0, such as padding, count
     neither in the loss nor in the counts made here.  The sums have a fixed order."""
     _check_logits(router_logits)
     T, E = router_logits.shape
@@ -650,14 +654,21 @@ def switch_loss(router_logits: torch.Tensor, expert_frequency: torch.Tensor = No
             raise ValueError(f"topk_indices must be [{T}, K], got {tuple(topk_indices.shape)}")
         K = topk_indices.shape[1]
     else:
-        _need(expert_frequency, "expert_frequency", torch.int32)
+        _need(expert_frequency, "expert_frequency")
+        if expert_frequency.dtype not in _COUNT_TYPES:
+            raise ValueError(f"expert_frequency must be int32, int64, fp32 or fp64, got {expert_frequency.dtype}")
         if tuple(expert_frequency.shape) != (E,):
             raise ValueError(f"expert_frequency must be [{E}], got {tuple(expert_frequency.shape)}")
     dev = router_logits.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    freq = torch.empty(E, dtype=torch.int32, device=dev)
     coef = torch.empty(E, dtype=torch.float32, device=dev)
     ws = _workspace(nat.load().sm_switch_loss_workspace(T, E), dev)
+    if expert_frequency is not None and expert_frequency.dtype != torch.int32:
+        _call_on(dev, "sm_switch_loss_counts", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E,
+                 _ptr(token_mask), _ptr(expert_frequency), _COUNT_TYPES[expert_frequency.dtype], _ptr(loss), _ptr(coef),
+                 _ptr(ws), ws.numel())
+        return loss, expert_frequency.clone(), coef
+    freq = torch.empty(E, dtype=torch.int32, device=dev)
     _call_on(dev, "sm_switch_loss", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E, _ptr(token_mask),
              _ptr(topk_indices), K, _ptr(expert_frequency), _ptr(loss), _ptr(coef), _ptr(freq), _ptr(ws), ws.numel(),
              _ptr(err))
