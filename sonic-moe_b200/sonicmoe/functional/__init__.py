@@ -628,6 +628,14 @@ def _given_counts(expert_frequency):
     return expert_frequency.to(dtype).contiguous()
 
 
+def _expert_ids(topk_indices, E):
+    if topk_indices.is_floating_point() or topk_indices.is_complex():
+        raise ValueError(f"topk_indices must hold whole numbers, got {topk_indices.dtype}")
+    if topk_indices.dtype == torch.int64:  # an id that int32 cannot hold must not become a valid one
+        topk_indices = topk_indices.clamp(-1, E)
+    return topk_indices.to(torch.int32).contiguous()
+
+
 def switch_load_balancing_loss(
     router_logits: torch.Tensor,
     expert_frequency: torch.Tensor | None = None,
@@ -655,7 +663,7 @@ def switch_load_balancing_loss(
     if expert_frequency is not None:
         expert_frequency = _given_counts(expert_frequency)
     if topk_indices is not None:
-        topk_indices = topk_indices.to(torch.int32).contiguous()
+        topk_indices = _expert_ids(topk_indices, router_logits.shape[-1])
     if token_mask is not None:
         token_mask = token_mask.contiguous()
     if torch.compiler.is_compiling():

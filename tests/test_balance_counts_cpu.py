@@ -38,6 +38,15 @@ def test_large_counts_do_not_wrap(seen):
     assert torch.equal(calls[0][0], f)
 
 
+def test_ids_that_int32_cannot_hold_stay_invalid(seen):
+    loss, calls = seen
+    ids = torch.tensor([[0, 3], [(1 << 32) + 1, -(1 << 32) + 2], [4, -1]])
+    loss(torch.zeros(3, 4), topk_indices=ids)
+    got = calls[0][1]
+    assert got.dtype == torch.int32 and got[0].tolist() == [0, 3]
+    assert ((got[1:] < 0) | (got[1:] >= 4)).all()
+
+
 def test_refusals(seen):
     loss, calls = seen
     z = torch.zeros(2, 3)
@@ -49,6 +58,8 @@ def test_refusals(seen):
             loss(z, expert_frequency=dual)
     with pytest.raises(ValueError, match="real numbers"):
         loss(z, expert_frequency=torch.ones(3, dtype=torch.complex64))
+    with pytest.raises(ValueError, match="whole numbers"):
+        loss(z, topk_indices=torch.zeros(2, 1))
     assert not calls
 
 
