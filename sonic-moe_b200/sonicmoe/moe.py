@@ -8,6 +8,7 @@ this package has no eager-torch or scattermoe execution path, and asking for one
 """
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from .enums import ActivationType, KernelBackendMoE, is_glu
 from .functional import moe_TC_softmax_topk_layer, prepare_int4_weights, switch_load_balancing_loss
@@ -121,5 +122,22 @@ class MoE(nn.Module):
         if is_inference_mode:
             aux_loss = None
         else:
-            aux_loss, _ = switch_load_balancing_loss(router_logits, expert_frequency)
+            # a subclass's or an instance's own loss gets the probabilities, which the kernels do not need
+            own = type(self)._compute_switch_loss is MoE._compute_switch_loss and \
+                "_compute_switch_loss" not in self.__dict__
+            aux_loss = self._compute_switch_loss(
+                logits=router_logits,
+                probs=None if own else F.softmax(router_logits, dim=-1, dtype=torch.float32),
+                expert_frequency=expert_frequency,
+            )
         return hidden_states, aux_loss
+
+    def _compute_switch_loss(self, logits, probs, expert_frequency):
+        """Switch load-balancing loss (reference moe.py:263-276).  With ``probs`` it is that of the given
+        probabilities, in torch operations; None stands for the softmax of the logits, by the kernels."""
+        logits = logits.view(-1, logits.size(-1))
+        if probs is None:
+            return switch_load_balancing_loss(logits, expert_frequency)[0]
+        acc_probs = probs.view(-1, probs.size(-1)).sum(0)
+        expert_frequency = expert_frequency.float()
+        return logits.size(1) * (F.normalize(acc_probs, p=1, dim=0) * F.normalize(expert_frequency, p=1, dim=0)).sum()
