@@ -22,8 +22,8 @@ Op boundary: as in the reference, the router top-k (``sonicmoe::_topk_fwd``,
 (``triton_kernels::TC_topk_router_metadata``, ``triton_kernels::general_routing_router_metadata``)
 are ``torch.library.custom_op``s writing into caller-allocated outputs; the engine's layer forward
 after the router GEMM is one more registered op per entry point (``sonicmoe::fp8_moe_tc_forward``,
-``sonicmoe::fp8_moe_general_forward``, with fake implementations for tracing), so ``torch.compile``
-traces a whole ``MoE`` forward without a graph break.
+``sonicmoe::fp8_moe_general_forward``, with fake implementations for tracing; the like for 4-bit weights), so
+``torch.compile`` traces a whole ``MoE`` forward without a graph break.
 
 Training: with ``is_inference_mode_enabled=False`` while autograd is recording and an input or
 weight requires grad, ``moe_TC_softmax_topk_layer`` and ``moe_general_routing_inputs`` run the
@@ -281,11 +281,26 @@ def _(x, router_scores, token_indices, expert_indices, w1, w2, concat_layout):
     return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(w2.shape[-1], dtype=torch.int32)
 
 
-def _int4_tc(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
-             is_softmax_over_topk, norm_topk_probs):
+def _int4_parts(w1, w2):
+    """A pair of prepared 4-bit weights taken apart, as the registered ops below take it."""
+    return w1.q, w1.scales, w2.q, w2.scales, list(w1.shape), list(w2.shape), w1.group_size, w2.group_size
+
+
+def _int4_whole(w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group):
+    # concat_glu only says how the caller's rows were ordered before they were prepared
+    return (Int4ExpertWeights(w1q, w1_scales, tuple(w1_shape), w1_group, False),
+            Int4ExpertWeights(w2q, w2_scales, tuple(w2_shape), w2_group, False))
+
+
+def _int4_tc(x, router_logits, w1, w2, K, is_softmax_over_topk, norm_topk_probs):
     scores, idx = ops.router_topk(router_logits, K, is_softmax_over_topk, norm_topk_probs)
-    return ops.moe_int4_forward(x, scores, idx, Int4ExpertWeights(w1q, w1_scales, tuple(w1_shape), w1_group, False),
-                                Int4ExpertWeights(w2q, w2_scales, tuple(w2_shape), w2_group, False))
+    return ops.moe_int4_forward(x, scores, idx, w1, w2)
+
+
+def _int4_tc_fused_router(x, router_w, w1, w2, K, is_softmax_over_topk, norm_topk_probs):
+    router_logits, scores, idx = ops.router_fused(x, router_w, K, is_softmax_over_topk, norm_topk_probs)
+    o, expert_frequency = ops.moe_int4_forward(x, scores, idx, w1, w2)
+    return o, router_logits, expert_frequency
 
 
 @torch.library.custom_op("sonicmoe::int4_moe_tc_forward", mutates_args=())
@@ -306,14 +321,69 @@ def _int4_moe_tc_forward(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``moe_TC_softmax_topk_layer`` after the router GEMM on 4-bit expert weights (the prepared
     ``Int4ExpertWeights`` taken apart): (o [T, H] bf16, expert_frequency [E] int32)."""
-    return _int4_tc(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
-                    is_softmax_over_topk, norm_topk_probs)
+    w1, w2 = _int4_whole(w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group)
+    return _int4_tc(x, router_logits, w1, w2, K, is_softmax_over_topk, norm_topk_probs)
 
 
 @_int4_moe_tc_forward.register_fake
 def _(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
       is_softmax_over_topk, norm_topk_probs):
     return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(router_logits.shape[1], dtype=torch.int32)
+
+
+@torch.library.custom_op("sonicmoe::int4_moe_tc_forward_fused_router", mutates_args=())
+def _int4_moe_tc_forward_fused_router(
+    x: torch.Tensor,
+    router_w: torch.Tensor,
+    w1q: torch.Tensor,
+    w1_scales: torch.Tensor,
+    w2q: torch.Tensor,
+    w2_scales: torch.Tensor,
+    w1_shape: list[int],
+    w2_shape: list[int],
+    w1_group: int,
+    w2_group: int,
+    K: int,
+    is_softmax_over_topk: bool,
+    norm_topk_probs: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The same with the fused router: (o [T, H] bf16, router_logits [T, E] bf16, expert_frequency [E] int32)."""
+    w1, w2 = _int4_whole(w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group)
+    return _int4_tc_fused_router(x, router_w, w1, w2, K, is_softmax_over_topk, norm_topk_probs)
+
+
+@_int4_moe_tc_forward_fused_router.register_fake
+def _(x, router_w, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group, K,
+      is_softmax_over_topk, norm_topk_probs):
+    E = router_w.shape[0]
+    return (x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty((x.shape[0], E), dtype=torch.bfloat16),
+            x.new_empty(E, dtype=torch.int32))
+
+
+@torch.library.custom_op("sonicmoe::int4_moe_general_forward", mutates_args=())
+def _int4_moe_general_forward(
+    x: torch.Tensor,
+    router_scores: torch.Tensor,
+    token_indices: torch.Tensor,
+    expert_indices: torch.Tensor,
+    w1q: torch.Tensor,
+    w1_scales: torch.Tensor,
+    w2q: torch.Tensor,
+    w2_scales: torch.Tensor,
+    w1_shape: list[int],
+    w2_shape: list[int],
+    w1_group: int,
+    w2_group: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``moe_general_routing_inputs`` on 4-bit expert weights: (o [T, H] bf16, expert_frequency [E] int32)."""
+    w1, w2 = _int4_whole(w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group, w2_group)
+    return ops.moe_int4_general_forward(x, router_scores, token_indices, expert_indices, w1, w2)
+
+
+@_int4_moe_general_forward.register_fake
+def _(x, router_scores, token_indices, expert_indices, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_group,
+      w2_group):
+    return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(w2_shape[0], dtype=torch.int32)
 
 
 class _FP8MoEGeneralFunction(torch.autograd.Function):
@@ -401,16 +471,18 @@ def moe_TC_softmax_topk_layer(
         x = x.to(torch.bfloat16)
     x = x.contiguous()
     if int4:
+        traced = torch.compiler.is_compiling()
+        modes = (K, is_softmax_over_topk, norm_topk_probs)
         if fused_router:
-            router_logits, scores, idx = ops.router_fused(x, router_w.to(x.dtype).contiguous(), K,
-                                                          is_softmax_over_topk, norm_topk_probs)
-            o, expert_frequency = ops.moe_int4_forward(x, scores, idx, w1, w2)
-            return o, router_logits, expert_frequency
+            rw = router_w.to(x.dtype).contiguous()
+            if traced:
+                return _int4_moe_tc_forward_fused_router(x, rw, *_int4_parts(w1, w2), *modes)
+            return _int4_tc_fused_router(x, rw, w1, w2, *modes)
         router_logits = F.linear(x, router_w.to(x.dtype))
-        layer = _int4_moe_tc_forward if torch.compiler.is_compiling() else _int4_tc
-        o, expert_frequency = layer(x, router_logits.contiguous(), w1.q, w1.scales, w2.q, w2.scales, list(w1.shape),
-                                    list(w2.shape), w1.group_size, w2.group_size, K, is_softmax_over_topk,
-                                    norm_topk_probs)
+        if traced:
+            o, expert_frequency = _int4_moe_tc_forward(x, router_logits.contiguous(), *_int4_parts(w1, w2), *modes)
+        else:
+            o, expert_frequency = _int4_tc(x, router_logits.contiguous(), w1, w2, *modes)
         return o, router_logits, expert_frequency
     if training:
         router_logits = F.linear(x, router_w.to(x.dtype))
@@ -480,6 +552,8 @@ def moe_general_routing_inputs(
     args = (x, router_scores.contiguous(), token_indices.to(torch.int32).contiguous(),
             expert_indices.to(torch.int32).contiguous())
     if int4:
+        if torch.compiler.is_compiling():
+            return _int4_moe_general_forward(*args, *_int4_parts(w1, w2))
         return ops.moe_int4_general_forward(*args, w1, w2)
     if training:
         return _FP8MoEGeneralFunction.apply(*args, w1, w2, concat_layout)
