@@ -38,11 +38,13 @@ covers ``moe_TC_softmax_topk_layer`` and ``moe_general_routing_inputs`` (both w1
 I % 256 == 0) -- the fused router and prepared e4m3 weights raise ``NotImplementedError`` when a
 gradient is requested, instead of returning an output whose weights would never receive one.
 """
+import itertools
 import weakref
 
 import torch
 import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from .. import ops
 from ..enums import ActivationType
@@ -124,6 +126,65 @@ def prepare_int4_weights(w: torch.Tensor, group_size: int = 128, concat_glu: boo
     given in the reference's (N, K, E) view.  Nothing is cached: the caller keeps the result."""
     with torch.no_grad():
         return ops.weight_prep_int4(_as_expert_major(w.detach()), group_size, concat_glu=concat_glu)
+
+
+class Int4Copies:
+    """4-bit copies of a module's expert weights w1 [E, 2I, H] and w2 [E, H, I], made again when a weight has changed:
+    another storage, address, shape or version counter (inference tensors have no counter, so there only the former).
+
+    Weights that were put away (None, empty, or on another kind of device than the copies) leave the copies in use,
+    unless they were changed first.  A deep or pickled copy of this object belongs to other weights and makes its own
+    at the first use."""
+
+    _known = weakref.WeakValueDictionary()  # for traced callers, which name it by its number
+    _numbers = itertools.count()
+
+    def __init__(self, group_size: int, copies=(None, None)):
+        self.group_size = group_size
+        self.copies = tuple(copies)
+        # apart from the copies themselves, which a traced caller must not depend on: they may be made again
+        self._on = None if self.copies[0] is None else self.copies[0].q.device.type
+        self._states = [None, None]
+        self.handle = next(self._numbers)
+        self._known[self.handle] = self
+
+    def __reduce__(self):
+        return Int4Copies, (self.group_size, self.copies)
+
+    @staticmethod
+    def _state(w):
+        storage = w.untyped_storage()
+        # the weak reference keeps a freed storage's identity from being given to another
+        return StorageWeakRef(storage), storage._cdata, w.data_ptr(), w.shape, w.dtype, \
+            None if w.is_inference() else w._version
+
+    def away(self, w1, w2) -> bool:
+        """A weight cannot be prepared, and there are copies to go on with."""
+        return self._on is not None and any(w is None or w.numel() == 0 or w.device.type != self._on for w in (w1, w2))
+
+    def current(self, w1, w2):
+        """The copies (w1's, w2's) of the weights as they are."""
+        weights = (w1, w2)
+        if self.away(w1, w2):
+            for w, state in zip(weights, self._states):
+                if w is not None and state is not None and not w.is_inference() and (state[-1] or 0) < w._version:
+                    raise RuntimeError("the expert weights were changed and put away since their 4-bit copies were made: "
+                                       "bring them back, or call use_int4_experts with them in place")
+            return self.copies
+        fresh = [self._fresh(w, s) for w, s in zip(weights, self._states)]
+        if not all(fresh):
+            self.copies = tuple(c if ok else prepare_int4_weights(w.permute(1, 2, 0), self.group_size)
+                                for w, c, ok in zip(weights, self.copies, fresh))
+            self._on = self.copies[0].q.device.type
+            self._states = [self._state(w) for w in weights]
+        return self.copies
+
+    def _fresh(self, w, state):
+        if state is None:
+            return False
+        _, storage, ptr, shape, dtype, version = state
+        return (w.data_ptr() == ptr and (w.is_inference() or w._version == version)
+                and w.untyped_storage()._cdata == storage and w.shape == shape and w.dtype == dtype)
 
 
 def _int4_pair(w1, w2, concat_layout) -> bool:
@@ -331,6 +392,25 @@ def _(x, router_logits, w1q, w1_scales, w2q, w2_scales, w1_shape, w2_shape, w1_g
     return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(router_logits.shape[1], dtype=torch.int32)
 
 
+@torch.library.custom_op("sonicmoe::int4_module_forward", mutates_args=())
+def _int4_module_forward(
+    x: torch.Tensor,
+    router_logits: torch.Tensor,
+    w1: torch.Tensor,
+    w2: torch.Tensor,
+    handle: int,
+    K: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The layer after the router GEMM on the ``Int4Copies`` of that number, of the module's weights w1 [E, 2I, H]
+    and w2 [E, H, I] as they are when the graph runs."""
+    return _int4_tc(x, router_logits, *Int4Copies._known[handle].current(w1, w2), K, True, False)
+
+
+@_int4_module_forward.register_fake
+def _(x, router_logits, w1, w2, handle, K):
+    return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(router_logits.shape[1], dtype=torch.int32)
+
+
 @torch.library.custom_op("sonicmoe::int4_moe_tc_forward_fused_router", mutates_args=())
 def _int4_moe_tc_forward_fused_router(
     x: torch.Tensor,
@@ -516,6 +596,22 @@ def moe_TC_softmax_topk_layer(
         o, expert_frequency = _fp8_moe_tc_forward(
             x, router_logits.contiguous(), w1, w2, K, is_softmax_over_topk, norm_topk_probs, concat_layout
         )
+    return o, router_logits, expert_frequency
+
+
+def int4_module_layer(x, router_w, w1, b1, w2, b2, K: int, copies: Int4Copies, activation_type=ActivationType.SWIGLU,
+                      is_inference_mode_enabled: bool = False):
+    """``moe_TC_softmax_topk_layer`` on the 4-bit copies of a module's weights w1 [E, 2I, H] and w2 [E, H, I], brought
+    up to date."""
+    if not torch.compiler.is_compiling() or copies.away(w1, w2):
+        q1, q2 = copies.copies if torch.compiler.is_compiling() else copies.current(w1, w2)
+        return moe_TC_softmax_topk_layer(x, router_w, q1, b1, q2, b2, K, None, activation_type, is_inference_mode_enabled)
+    _check_common(b1, b2, activation_type)
+    if _wants_training(is_inference_mode_enabled, x, router_w):
+        raise NotImplementedError("4-bit expert weights have no backward")
+    x = x.to(torch.bfloat16).contiguous()
+    router_logits = F.linear(x, router_w.to(x.dtype))
+    o, expert_frequency = _int4_module_forward(x, router_logits.contiguous(), w1.detach(), w2.detach(), copies.handle, K)
     return o, router_logits, expert_frequency
 
 

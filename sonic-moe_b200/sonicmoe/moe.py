@@ -11,7 +11,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .enums import ActivationType, KernelBackendMoE, is_glu
-from .functional import moe_TC_softmax_topk_layer, prepare_int4_weights, switch_load_balancing_loss
+from .functional import Int4Copies, int4_module_layer, moe_TC_softmax_topk_layer, switch_load_balancing_loss
 
 
 class Experts(nn.Module):
@@ -81,13 +81,15 @@ class MoE(nn.Module):
         """Run inference forwards on 4-bit copies of the present expert weights, with a scale per
         ``group_size`` (32, 64 or 128) input columns; None goes back to the FP8 engine.
 
-        The copies are made here, on the weights' device, and kept: after changing the weights or moving the
-        module, call it again.  A forward that needs gradients raises NotImplementedError meanwhile."""
+        The copies are made here, on the weights' device, and made again by a forward that finds a weight changed,
+        replaced or moved to another GPU.  Weights put away afterwards to save memory (None, emptied, on the CPU)
+        leave the copies in use.  A forward that needs gradients raises NotImplementedError meanwhile."""
         if group_size is None:
             self._int4_experts = None
         else:
-            self._int4_experts = tuple(prepare_int4_weights(w.weight.permute(1, 2, 0), group_size)
-                                       for w in (self.c_fc, self.c_proj))
+            copies = Int4Copies(group_size)
+            copies.current(self.c_fc.weight, self.c_proj.weight)
+            self._int4_experts = copies
         return self
 
     def forward(
@@ -100,24 +102,35 @@ class MoE(nn.Module):
             raise NotImplementedError(
                 f"backend {kernel_backend_moe} is not provided by the B200 engine; use KernelBackendMoE.sonicmoe"
             )
-        if self._int4_experts is not None:
-            w1, w2 = self._int4_experts
-        else:
-            w1, w2 = self.c_fc.weight.permute(1, 2, 0), self.c_proj.weight.permute(1, 2, 0)
         original_shape = hidden_states.shape
         hidden_states = hidden_states.view(-1, self.hidden_size)
-        hidden_states, router_logits, expert_frequency = moe_TC_softmax_topk_layer(
-            hidden_states,
-            self.router.weight,
-            w1,
-            self.c_fc.bias,
-            w2,
-            self.c_proj.bias,
-            self.top_k,
-            self.stream_id,
-            self.activation_function,
-            is_inference_mode or not self.training,
-        )
+        inference = is_inference_mode or not self.training
+        if self._int4_experts is not None:
+            hidden_states, router_logits, expert_frequency = int4_module_layer(
+                hidden_states,
+                self.router.weight,
+                self.c_fc.weight,
+                self.c_fc.bias,
+                self.c_proj.weight,
+                self.c_proj.bias,
+                self.top_k,
+                self._int4_experts,
+                self.activation_function,
+                inference,
+            )
+        else:
+            hidden_states, router_logits, expert_frequency = moe_TC_softmax_topk_layer(
+                hidden_states,
+                self.router.weight,
+                self.c_fc.weight.permute(1, 2, 0),
+                self.c_fc.bias,
+                self.c_proj.weight.permute(1, 2, 0),
+                self.c_proj.bias,
+                self.top_k,
+                self.stream_id,
+                self.activation_function,
+                inference,
+            )
         hidden_states = hidden_states.view(original_shape)
         if is_inference_mode:
             aux_loss = None
