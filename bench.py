@@ -646,6 +646,8 @@ def main():
                     help="only run warmup + steps eager forwards (no graph, baselines or extra timing), "
                          "for ncu captures; prints nothing")
     args = ap.parse_args()
+    if args.expert_bits == 4 and not args.workload.startswith("c5"):
+        ap.error("--expert-bits 4 is for the decoding workloads c5_64 and c5_512")
     CFG["T"] = args.tokens
     EP_WORKLOADS["c2"]["T"] = args.tokens
     if args.warmup < 3:
