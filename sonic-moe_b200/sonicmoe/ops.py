@@ -50,19 +50,8 @@ def router_topk(router_logits: torch.Tensor, K: int, softmax_over_topk: bool = T
     _need(idx, "idx", torch.int32)
     if tuple(scores.shape) != (T, K) or tuple(idx.shape) != (T, K):
         raise ValueError(f"outputs must be [{T}, {K}]")
-    nat.call(
-        "sm_router_topk",
-        _ptr(router_logits),
-        _LOGIT_DTYPES[router_logits.dtype],
-        T,
-        E,
-        K,
-        int(softmax_over_topk),
-        int(norm_topk_probs),
-        _ptr(scores),
-        _ptr(idx),
-        _stream(),
-    )
+    _call_on(router_logits.device, "sm_router_topk", _ptr(router_logits), _LOGIT_DTYPES[router_logits.dtype], T, E, K,
+             int(softmax_over_topk), int(norm_topk_probs), _ptr(scores), _ptr(idx))
     return scores, idx
 
 
@@ -86,8 +75,8 @@ def router_fused(x: torch.Tensor, router_w: torch.Tensor, K: int, softmax_over_t
     if err is None:
         err = torch.zeros(1, dtype=torch.int32, device=dev)
     ws = _workspace(nat.load().sm_router_fused_workspace(T, E), dev)
-    nat.call("sm_router_fused", _ptr(x), _ptr(router_w), T, H, E, K, int(softmax_over_topk), int(norm_topk_probs),
-             _ptr(logits), _ptr(scores), _ptr(idx), _ptr(ws), ws.numel(), _ptr(err), _stream())
+    _call_on(dev, "sm_router_fused", _ptr(x), _ptr(router_w), T, H, E, K, int(softmax_over_topk), int(norm_topk_probs),
+             _ptr(logits), _ptr(scores), _ptr(idx), _ptr(ws), ws.numel(), _ptr(err))
     return logits, scores, idx
 
 
