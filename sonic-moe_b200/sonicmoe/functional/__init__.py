@@ -121,11 +121,13 @@ def prepare_fp8_weights(w, concat_glu: bool = False, with_t: bool = False) -> Fp
     return prepared
 
 
-def prepare_int4_weights(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False) -> Int4ExpertWeights:
+def prepare_int4_weights(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False,
+                         out: Int4ExpertWeights | None = None) -> Int4ExpertWeights:
     """4-bit version, with a scale per ``group_size`` (32, 64 or 128) input columns, of an expert weight
-    given in the reference's (N, K, E) view.  Nothing is cached: the caller keeps the result."""
+    given in the reference's (N, K, E) view.  Nothing is cached: the caller keeps the result.  ``out``: an
+    earlier result of the same shape, group and layout, whose buffers are written again."""
     with torch.no_grad():
-        return ops.weight_prep_int4(_as_expert_major(w.detach()), group_size, concat_glu=concat_glu)
+        return ops.weight_prep_int4(_as_expert_major(w.detach()), group_size, concat_glu=concat_glu, out=out)
 
 
 class Int4Copies:
@@ -134,7 +136,11 @@ class Int4Copies:
 
     Weights that were put away (None, empty, or on another kind of device than the copies) leave the copies in use,
     unless they were changed first.  A deep or pickled copy of this object belongs to other weights and makes its own
-    at the first use."""
+    at the first use.
+
+    New copies go into the old ones' buffers, which a captured graph may still read, and are complete on every stream
+    when they are given out (the device is waited for before and after).  A capture that finds a weight changed records
+    the preparation, of copies of its own."""
 
     _known = weakref.WeakValueDictionary()  # for traced callers, which name it by its number
     _numbers = itertools.count()
@@ -162,8 +168,8 @@ class Int4Copies:
         """A weight cannot be prepared, and there are copies to go on with."""
         return self._on is not None and any(w is None or w.numel() == 0 or w.device.type != self._on for w in (w1, w2))
 
-    def current(self, w1, w2):
-        """The copies (w1's, w2's) of the weights as they are."""
+    def current(self, w1, w2, again: bool = False):
+        """The copies (w1's, w2's) of the weights as they are; again: made again in any case."""
         weights = (w1, w2)
         if self.away(w1, w2):
             for w, state in zip(weights, self._states):
@@ -171,12 +177,28 @@ class Int4Copies:
                     raise RuntimeError("the expert weights were changed and put away since their 4-bit copies were made: "
                                        "bring them back, or call use_int4_experts with them in place")
             return self.copies
-        fresh = [self._fresh(w, s) for w, s in zip(weights, self._states)]
+        fresh = [not again and self._fresh(w, s) for w, s in zip(weights, self._states)]
         if not all(fresh):
-            self.copies = tuple(c if ok else prepare_int4_weights(w.permute(1, 2, 0), self.group_size)
-                                for w, c, ok in zip(weights, self.copies, fresh))
-            self._on = self.copies[0].q.device.type
-            self._states = [self._state(w) for w in weights]
+            return self._make(weights, fresh)
+        return self.copies
+
+    def _make(self, weights, fresh):
+        cuda = all(w.is_cuda for w in weights)
+        if cuda and torch.cuda.is_current_stream_capturing():  # nothing to keep of launches that have not run
+            return tuple(c if ok else prepare_int4_weights(w.permute(1, 2, 0), self.group_size)
+                         for w, c, ok in zip(weights, self.copies, fresh))
+        if cuda:
+            torch.cuda.synchronize(weights[0].device)
+        states = [self._state(w) for w in weights]
+        self._states = [None, None]
+        self.copies = tuple(c if ok else prepare_int4_weights(
+            w.permute(1, 2, 0), self.group_size,
+            out=c if c is not None and c.shape == tuple(w.shape) and c.q.device == w.device else None)
+            for w, c, ok in zip(weights, self.copies, fresh))
+        if cuda:
+            torch.cuda.synchronize(weights[0].device)
+        self._on = self.copies[0].q.device.type
+        self._states = states
         return self.copies
 
     def _fresh(self, w, state):

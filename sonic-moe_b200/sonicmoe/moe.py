@@ -82,13 +82,16 @@ class MoE(nn.Module):
         ``group_size`` (32, 64 or 128) input columns; None goes back to the FP8 engine.
 
         The copies are made here, on the weights' device, and made again by a forward that finds a weight changed,
-        replaced or moved to another GPU.  Weights put away afterwards to save memory (None, emptied, on the CPU)
+        replaced or moved to another GPU (a captured graph looks at no weight: it runs on the copies as the last such
+        forward or call of this method left them).  Weights put away afterwards to save memory (None, emptied, on the CPU)
         leave the copies in use.  A forward that needs gradients raises NotImplementedError meanwhile."""
         if group_size is None:
             self._int4_experts = None
         else:
-            copies = Int4Copies(group_size)
-            copies.current(self.c_fc.weight, self.c_proj.weight)
+            copies = self._int4_experts
+            if copies is None or copies.group_size != group_size:
+                copies = Int4Copies(group_size)
+            copies.current(self.c_fc.weight, self.c_proj.weight, again=True)
             self._int4_experts = copies
         return self
 

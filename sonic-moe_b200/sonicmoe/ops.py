@@ -697,9 +697,11 @@ class Int4ExpertWeights:
     concat_glu: bool
 
 
-def weight_prep_int4(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False) -> Int4ExpertWeights:
+def weight_prep_int4(w: torch.Tensor, group_size: int = 128, concat_glu: bool = False,
+                     out: Int4ExpertWeights = None) -> Int4ExpertWeights:
     """Quantise expert weights [E, N, K] (bf16) to codes in [-7, 7] with a scale per ``group_size`` (32,
-    64 or 128) input columns: the smallest number of 5 significant bits that is >= amax / 7."""
+    64 or 128) input columns: the smallest number of 5 significant bits that is >= amax / 7.  ``out``: an earlier
+    result of the same shape, group and layout to write into."""
     if w.dim() != 3:
         raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
     if w.dtype != torch.bfloat16:
@@ -708,10 +710,18 @@ def weight_prep_int4(w: torch.Tensor, group_size: int = 128, concat_glu: bool = 
     _need(w, "w", torch.bfloat16)
     E, N, K = w.shape
     lib = nat.load()
-    q = torch.empty(lib.sm_int4_weight_bytes(E, N, K), dtype=torch.uint8, device=w.device)
-    scales = torch.empty(lib.sm_int4_scale_count(E, N, K, group_size), dtype=torch.bfloat16, device=w.device)
-    _call_on(w.device, "sm_weight_prep_int4", _ptr(w), E, N, K, group_size, int(concat_glu), _ptr(q), _ptr(scales))
-    return Int4ExpertWeights(q, scales, (E, N, K), group_size, bool(concat_glu))
+    if out is None:
+        q = torch.empty(lib.sm_int4_weight_bytes(E, N, K), dtype=torch.uint8, device=w.device)
+        scales = torch.empty(lib.sm_int4_scale_count(E, N, K, group_size), dtype=torch.bfloat16, device=w.device)
+        out = Int4ExpertWeights(q, scales, (E, N, K), group_size, bool(concat_glu))
+    else:
+        if tuple(out.shape) != (E, N, K) or out.group_size != group_size or out.concat_glu != bool(concat_glu):
+            raise ValueError(f"out is of a weight {tuple(out.shape)} with a group of {out.group_size}")
+        _check_int4(out, "out")
+        _same_device(w, out=out.q, out_scales=out.scales)
+    _call_on(w.device, "sm_weight_prep_int4", _ptr(w), E, N, K, group_size, int(concat_glu), _ptr(out.q),
+             _ptr(out.scales))
+    return out
 
 
 def _check_int4(w: Int4ExpertWeights, name: str):
