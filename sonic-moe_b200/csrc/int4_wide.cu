@@ -28,10 +28,11 @@
 // an expert's token chunks follow each other, so their second reading of the weights is from L2.  kN is
 // 64 or 128; 128 halves the dequantising per token, 64 leaves room for a third stage of weights in tensor
 // memory.
-// What bounds it (512 tokens, 64 experts of 4096 x 1024): the dequantising warps.  Per SM a step of 256
+// What it spends its time on (512 tokens, 64 experts of 4096 x 1024): the dequantising warps.  Per SM a step of 256
 // rows takes about 1000 cycles, against 790 for its bytes at the HBM rate and 512 for its MMAs; 7 of the 11
 // instructions for 8 weights are integer ones, which an SM issues at half rate (448 cycles of the step).
-// The schedulers issue in 62% of the cycles, the integer pipe is busy in 57% of them.  24 dequantising warps
+// The schedulers issue in 62% of the cycles, the integer pipe is busy in 57% of them: no unit is full, the warps
+// also wait for their stores to tensor memory.  24 dequantising warps
 // gain nothing (16 tokens 167 against 163 us, 64 tokens 235 against 228).
 // Fetching the codes by bulk copies from a warp of their own instead of per-lane copies, which takes a
 // tenth of the instructions away but adds a barrier wait to every step, measured 117 us against 104 (up
@@ -118,7 +119,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop, where));
 }
 
-// Tokens of one of an expert's ceil(n / kN) chunks: equal shares, whole 16s but for the last.
+// Tokens of one of an expert's ceil(n / kN) chunks: the equal share rounded up to whole 16s, and what is left for
+// the last (193 tokens in chunks of 64: 64, 64, 64 and 1).
 __device__ __forceinline__ int wd_share(int n, int chunks) { return ((n + chunks - 1) / chunks + 15) & ~15; }
 
 // Place of column k (< 32) of a block of 32 in the permuted order.
