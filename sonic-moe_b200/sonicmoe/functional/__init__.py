@@ -147,12 +147,17 @@ class Int4Copies:
 
     def __init__(self, group_size: int, copies=(None, None)):
         self.group_size = group_size
-        self.copies = tuple(copies)
+        # the copies and the states of the weights they were made from: one value, so that a thread never sees the
+        # one without the other
+        self._now = tuple(copies), (None, None)
         # apart from the copies themselves, which a traced caller must not depend on: they may be made again
-        self._on = None if self.copies[0] is None else self.copies[0].q.device.type
-        self._states = [None, None]
+        self._on = None if copies[0] is None else copies[0].q.device.type
         self.handle = next(self._numbers)
         self._known[self.handle] = self
+
+    @property
+    def copies(self):
+        return self._now[0]
 
     def __reduce__(self):
         return Int4Copies, (self.group_size, self.copies)
@@ -170,36 +175,33 @@ class Int4Copies:
 
     def current(self, w1, w2, again: bool = False):
         """The copies (w1's, w2's) of the weights as they are; again: made again in any case."""
-        weights = (w1, w2)
+        weights, (copies, states) = (w1, w2), self._now
         if self.away(w1, w2):
-            for w, state in zip(weights, self._states):
+            for w, state in zip(weights, states):
                 if w is not None and state is not None and not w.is_inference() and (state[-1] or 0) < w._version:
                     raise RuntimeError("the expert weights were changed and put away since their 4-bit copies were made: "
                                        "bring them back, or call use_int4_experts with them in place")
-            return self.copies
-        fresh = [not again and self._fresh(w, s) for w, s in zip(weights, self._states)]
-        if not all(fresh):
-            return self._make(weights, fresh)
-        return self.copies
+            return copies
+        fresh = [not again and self._fresh(w, s) for w, s in zip(weights, states)]
+        return copies if all(fresh) else self._make(weights, copies, fresh)
 
-    def _make(self, weights, fresh):
+    def _make(self, weights, copies, fresh):
         cuda = all(w.is_cuda for w in weights)
         if cuda and torch.cuda.is_current_stream_capturing():  # nothing to keep of launches that have not run
             return tuple(c if ok else prepare_int4_weights(w.permute(1, 2, 0), self.group_size)
-                         for w, c, ok in zip(weights, self.copies, fresh))
+                         for w, c, ok in zip(weights, copies, fresh))
         if cuda:
             torch.cuda.synchronize(weights[0].device)
-        states = [self._state(w) for w in weights]
-        self._states = [None, None]
-        self.copies = tuple(c if ok else prepare_int4_weights(
+        states = tuple(self._state(w) for w in weights)
+        self._now = copies, (None, None)
+        made = tuple(c if ok else prepare_int4_weights(
             w.permute(1, 2, 0), self.group_size,
             out=c if c is not None and c.shape == tuple(w.shape) and c.q.device == w.device else None)
-            for w, c, ok in zip(weights, self.copies, fresh))
+            for w, c, ok in zip(weights, copies, fresh))
         if cuda:
             torch.cuda.synchronize(weights[0].device)
-        self._on = self.copies[0].q.device.type
-        self._states = states
-        return self.copies
+        self._now, self._on = (made, states), made[0].q.device.type
+        return made
 
     def _fresh(self, w, state):
         if state is None:
